@@ -5,7 +5,10 @@
 
 No CMake: one hipcc invocation per translation unit, then a shared link.  `-ffp-contract=off`
 keeps every multiply and add separately rounded, the same operation sequence as the reference's
-CPU ATen path, so boundary decisions (OOB / mask / argmin) agree with it.
+CPU ATen path, so boundary decisions (OOB / mask / argmin) agree with it.  Packed fp32 instructions
+are off: the compiler forms them from ordinary float code, and some of their forms have returned
+wrong values on this hardware without an error (the host pass warns that it does not know the
+feature: harmless).
 """
 import hashlib
 import os
@@ -20,6 +23,7 @@ LIB = os.path.join(HERE, 'libvfd_hip.so')
 SOURCES = ['capi.hip', 'fusion.hip', 'view.hip', 'photo.hip', 'aggregate.hip', 'projconv.hip', 'depthsyn.hip', 'padconv.hip', 'bnact.hip', 'reflectpad.hip', 'geometry.hip', 'maxpool.hip', 'weights.hip', 'dispconv.hip', 'decconv.hip']
 ARCH = os.environ.get('VFD_OFFLOAD_ARCH', 'gfx950')
 FLAGS = ['-O3', f'--offload-arch={ARCH}', '-std=c++17', '-fPIC', '-ffp-contract=off',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-Wno-unused-result', '-I', INCLUDE, '-I', CSRC]
 
 
