@@ -578,13 +578,71 @@ int vfd_aggregate_bwd(int BN, int C, int h, int w, const float* g, const float* 
 int vfd_upsample_ac_bwd(const float* g, float* dsrc, float* tmp, long long planes, int h, int w, int hs, int ws,
                         void* stream);
 
+/* ------------------------------------------------------------------ layer norm */
+typedef struct vfd_norm_desc {
+  int32_t rows, cols;    /* normalised over the cols (1 .. 2^28) values of each row               */
+  int64_t ldx;           /* elements from one row of x to the next (>= cols); the others are dense */
+  float eps;
+  int32_t dtype;         /* of x, y, g, dx: 0 fp32, 1 bf16                                         */
+} vfd_norm_desc;
+
+/* y = (x - mean) * rstd * w + b per row, rstd = 1 / sqrt(biased variance + eps); w, b fp32 [cols], null = 1, 0;
+ * mean, rstd fp32 [rows] for the backward (both or neither null).  Rows start at any element boundary. */
+int vfd_layer_norm_fwd(const vfd_norm_desc* d, const void* x, const float* w, const float* b, void* y, float* mean,
+                       float* rstd, void* stream);
+/* dx [rows, cols], dw [cols], db [cols] (each null = not computed; dw, db fp32) from g [rows, cols] and the forward's
+ * x, mean, rstd.  Column sums in a fixed order through the workspace (needed for dw / db). */
+size_t vfd_layer_norm_bwd_workspace(const vfd_norm_desc* d);
+int vfd_layer_norm_bwd(const vfd_norm_desc* d, const void* g, const void* x, const float* w, const float* mean,
+                       const float* rstd, void* dx, float* dw, float* db, void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ linear layer with epilogue */
+#define VFD_LINEAR_MAX (1 << 30)
+typedef struct vfd_linear_desc {
+  int32_t rows, k, n;    /* x [rows, k], w [n, k], y [rows, n]; each 0 .. VFD_LINEAR_MAX            */
+  int32_t act;           /* 0 none, 1 ReLU, 2 LeakyReLU(0.1), 3 ELU, 4 GELU (erf), 5 SiLU           */
+  int64_t ldx;           /* elements from one row of x to the next (>= k); all others are dense     */
+  int32_t dtype;         /* of every tensor: 0 fp32, 1 bf16 (sums fp32, outputs rounded once)       */
+} vfd_linear_desc;
+enum { VFD_LINEAR_FWD = 0, VFD_LINEAR_DGRAD = 1, VFD_LINEAR_WGRAD = 2, VFD_LINEAR_ACT_BWD = 3 };
+
+/* Workspace bytes of one of the calls below (0 = none needed). */
+size_t vfd_linear_workspace(const vfd_linear_desc* d, int what);
+/* y = act(x w^T + bias) + res; bias [n], res [rows, n] and z (the pre-activation, kept for the backward) may be null. */
+int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z,
+                   void* workspace, size_t ws_bytes, void* stream);
+/* gz = g act'(z) [rows, n] (act 0: gz is g, z and gz are not used) and db [n] = its column sums (null: not computed). */
+int vfd_linear_act_bwd(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, void* workspace,
+                       size_t ws_bytes, void* stream);
+/* dx [rows, k] = gz w */
+int vfd_linear_dgrad(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, void* workspace, size_t ws_bytes,
+                     void* stream);
+/* dw [n, k] = gz^T x */
+int vfd_linear_wgrad(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, void* workspace, size_t ws_bytes,
+                     void* stream);
+
+/* ------------------------------------------------------------------ gradient norm / clipping */
+/* Global norm of n gradient tensors (grads[i]: device pointer of numel[i] densely stored elements at any element
+ * boundary, dtypes[i] 0 fp32 / 1 bf16; the three arrays are host memory, read before the call returns):
+ * norm (one fp32 on the device) = sqrt(sum of all squares), or with inf_norm the largest magnitude (NaN if any is
+ * NaN).  Sums in fp64, fixed order.  n = 0: norm = 0. */
+size_t vfd_grad_norm_workspace(int n, const int64_t* numel);
+int vfd_grad_norm(int n, const void* const* grads, const int64_t* numel, const uint8_t* dtypes, int inf_norm, float* norm,
+                  void* workspace, size_t ws_bytes, void* stream);
+/* As vfd_grad_norm, and every gradient times c = min(1, max_norm / (norm + 1e-6)) (NaN for a NaN norm): in place
+ * (outs null; untouched when c == 1), or into outs[i] (numel[i] elements of out_dtypes[i]) with grads[i] left as it
+ * is.  No output may overlap a gradient or another output (in place: no two gradients may overlap). */
+int vfd_clip_grads(int n, const void* const* grads, const int64_t* numel, const uint8_t* dtypes, int inf_norm, double max_norm,
+                   void* const* outs, const uint8_t* out_dtypes, float* norm, void* workspace, size_t ws_bytes,
+                   void* stream);
+
 /* ------------------------------------------------------------------ measurement hooks */
 /* Record HIP events around every launch of kernel `kernel_id` (see vfd_kernel_name; -1 = all,
  * -2 = off) on the launching stream.  vfd_prof_read: launches and summed ms of everything
  * recorded; vfd_prof_read_kernels: the same per kernel id into arrays of `count` entries.
  * Both reset the record. */
 #define VFD_PROF_ALL (-1)
-#define VFD_KERNEL_COUNT 33
+#define VFD_KERNEL_COUNT 39
 const char* vfd_kernel_name(int kernel_id);
 int vfd_prof_enable(int kernel_id);
 int vfd_prof_read(int* launches, double* total_ms);

@@ -1,0 +1,384 @@
+"""Linear layer with bias, activation and residual in the product's epilogue (linear.hip, kernels.LinearAct,
+layers.linear_act), forward and backward.
+
+Tolerances (u = 2^-24, h = the type's half step): a product over K values is off by at most (K + 8) u sum|a b| in any
+order of summation (products of bf16 values are exact in 32 bits); an activation adds its slope's bound times that and
+8 u (|z| + 1) of its own; the backward reads the pre-activation rounded to the type (h |z|), which moves a slope by its
+Lipschitz constant times that, and the products take the gradient behind the activation rounded to the type (h |gz|).
+Where a pre-activation lies within its own error of the kink of relu or lrelu, either slope is right.  Each output is
+rounded once."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+F32, BF16 = torch.float32, torch.bfloat16
+U = 2.0 ** -24
+HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8}
+TINY = 2.0 ** -126
+ACTS = ['none', 'relu', 'lrelu', 'elu', 'gelu', 'silu']
+
+
+def _slope(z, act):
+    """(value, slope, bound of the slope's own slope) in 64 bits."""
+    one = torch.ones_like(z)
+    if act == 'none':
+        return z, one, 0.0
+    if act == 'relu':
+        return z.clamp_min(0), (z > 0).double(), 0.0
+    if act == 'lrelu':
+        s = torch.where(z > 0, one, 0.1 * one)
+        return z * s, s, 0.0
+    if act == 'elu':
+        n = z.clamp_max(0)
+        return torch.where(z > 0, z, torch.expm1(n)), torch.exp(n), 1.0
+    if act == 'gelu':
+        c = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi), 0.8
+    s = torch.sigmoid(z)
+    return z * s, s * (1 + z * (1 - s)), 0.5
+
+
+def _case(M, K, N, dtype, bias=True, residual=True, seed=0, device='cuda'):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, w, b, res, g = r(M, K), r(N, K) * K ** -0.5, r(N) * 0.3, r(M, N), r(M, N)
+    return [t.to(dtype).to(device) if t is not None else None
+            for t in (x, w, b if bias else None, res if residual else None, g)]
+
+
+def _oracle(x, w, b, res, g, act):
+    """Values and allowed errors (before the output's rounding) of y, dx, dw, db, dr."""
+    hT = HALF[x.dtype]
+    x, w, b, res, g = (None if t is None else t.detach().cpu().double() for t in (x, w, b, res, g))
+    M, K = x.shape
+    N = w.shape[0]
+    z = x @ w.t()
+    dz = (K + 8) * U * (x.abs() @ w.abs().t())
+    if b is not None:
+        z = z + b
+        dz = dz + U * z.abs()
+    a, s, lip = _slope(z, act)
+    y = a if res is None else a + res
+    ey = 1.13 * dz + (8 * U * (z.abs() + 1) if act != 'none' else 0) + U * y.abs()
+    gz = g * s
+    es = lip * (dz + hT * z.abs()) + 8 * U
+    if act in ('relu', 'lrelu'):
+        es = es + (z.abs() <= dz).double()
+    eg = g.abs() * es + U * gz.abs() if act != 'none' else torch.zeros_like(gz)
+    er = eg + (hT * (gz.abs() + eg) if act != 'none' else 0)
+    vals = [y, gz @ w, gz.t() @ x, gz.sum(0), g]
+    tol = [ey, er @ w.abs() + (N + 8) * U * (gz.abs() @ w.abs()), er.t() @ x.abs() + (M + 8) * U * (gz.abs().t() @ x.abs()),
+           eg.sum(0) + (M / 64 + 60) * U * gz.abs().sum(0), torch.zeros_like(g)]
+    return vals, tol
+
+
+def _check(got, vals, tol):
+    for t, v, e, name in zip(got, vals, tol, ('y', 'dx', 'dw', 'db', 'dr')):
+        if t is None:
+            continue
+        err = (t.detach().cpu().double() - v).abs()
+        lim = e + HALF[t.dtype] * (v.abs() + e) + TINY
+        assert t.shape == v.shape and bool((err <= lim).all()), (name, float((err / lim).max()))
+
+
+def _run(x, w, b, res, g, act):
+    from vfdepth_amd import kernels as KN
+    leaves = [t.requires_grad_(True) for t in (x, w, b, res) if t is not None]
+    y = KN.LinearAct.apply(x, w, b, res, act)
+    grads = iter(torch.autograd.grad(y, leaves, g))
+    return [y] + [next(grads) if t is not None else None for t in (x, w, b, res)]
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+def _desc(rows=4, k=8, n=8, act=0, ldx=8, dtype=0):
+    from vfdepth_amd import _lib
+    return _lib.LinearDesc(rows, k, n, act, ldx, dtype)
+
+
+@pytest.mark.parametrize('bad', [dict(rows=-1), dict(k=-1), dict(n=-2), dict(act=6), dict(act=-1), dict(ldx=7), dict(dtype=2),
+                                 dict(rows=(1 << 30) + 1), dict(rows=1 << 30, n=1 << 30)])
+def test_c_refuses_bad_descriptors(bad):
+    from vfdepth_amd import _lib
+    lib = _lib.load()
+    d = _desc(**bad)
+    p = 1 << 40
+    for rc in (lib.vfd_linear_fwd(ctypes.byref(d), p, p, p, p, p, p, p, 1 << 40, None),
+               lib.vfd_linear_act_bwd(ctypes.byref(d), p, p, p, p, p, 1 << 40, None),
+               lib.vfd_linear_dgrad(ctypes.byref(d), p, p, p, p, 1 << 40, None),
+               lib.vfd_linear_wgrad(ctypes.byref(d), p, p, p, p, 1 << 40, None)):
+        assert rc == -1 and (b'descriptor' in lib.vfd_last_error() or b'tiles' in lib.vfd_last_error())
+    assert lib.vfd_linear_workspace(ctypes.byref(d), 0) == 0
+
+
+def test_c_refuses_null_tensors_and_small_workspaces():
+    from vfdepth_amd import _lib
+    lib = _lib.load()
+    p = 1 << 40
+    d = _desc()
+    assert lib.vfd_linear_fwd(ctypes.byref(d), None, p, None, None, p, None, p, 1 << 40, None) == -1
+    assert lib.vfd_linear_fwd(ctypes.byref(d), p, p, None, None, None, None, p, 1 << 40, None) == -1
+    assert lib.vfd_linear_dgrad(ctypes.byref(d), p, None, p, p, 1 << 40, None) == -1
+    assert lib.vfd_linear_wgrad(ctypes.byref(d), p, p, None, p, 1 << 40, None) == -1
+    d = _desc(act=4)
+    assert lib.vfd_linear_act_bwd(ctypes.byref(d), p, None, p, p, p, 1 << 40, None) == -1
+    d = _desc(rows=100000, k=128, n=128, ldx=128)
+    need = lib.vfd_linear_workspace(ctypes.byref(d), _lib.LINEAR_WGRAD)
+    assert need > 0 and lib.vfd_linear_wgrad(ctypes.byref(d), p, p, p, p, need - 1, None) == -1
+    assert b'workspace' in lib.vfd_last_error()
+    need = lib.vfd_linear_workspace(ctypes.byref(d), _lib.LINEAR_ACT_BWD)
+    assert need > 0 and lib.vfd_linear_act_bwd(ctypes.byref(d), p, p, p, p, p, need - 1, None) == -1
+    for d in (_desc(rows=0), _desc(n=0)):                                        # nothing to do: nothing is launched
+        assert lib.vfd_linear_fwd(ctypes.byref(d), *[None] * 7, 0, None) == 0
+
+
+def test_descriptor_layout(tmp_path):
+    import os
+    import subprocess
+    from vfdepth_amd import _lib
+    src = tmp_path / 'sz.c'
+    src.write_text('#include "vfd_capi.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(){printf("%zu %zu %zu %zu", '
+                   'sizeof(vfd_linear_desc), offsetof(vfd_linear_desc, act), offsetof(vfd_linear_desc, ldx), '
+                   'offsetof(vfd_linear_desc, dtype)); return 0;}\n')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.check_call(['gcc', '-I', os.path.join(root, 'include'), str(src), '-o', str(tmp_path / 'sz')])
+    got = [int(v) for v in subprocess.check_output([str(tmp_path / 'sz')]).split()]
+    D = _lib.LinearDesc
+    assert got == [ctypes.sizeof(D), D.act.offset, D.ldx.offset, D.dtype.offset]
+
+
+@pytest.mark.parametrize('act', ACTS)
+def test_cpu_takes_the_module(act):
+    from vfdepth_amd import layers
+    torch.manual_seed(0)
+    lin, conv = torch.nn.Linear(5, 7).double(), torch.nn.Conv2d(5, 7, 1).double()
+    x, r = torch.randn(2, 3, 5).double(), torch.randn(2, 3, 7).double()
+    want = _slope(x @ lin.weight.t() + lin.bias, act)[0] + r
+    assert torch.allclose(layers.linear_act(lin, x, act, r), want, rtol=1e-12, atol=1e-12)
+    m = torch.randn(2, 5, 3, 4).double()
+    want = _slope(torch.einsum('nkhw,ok->nohw', m, conv.weight[:, :, 0, 0]) + conv.bias[:, None, None], act)[0]
+    assert torch.allclose(layers.linear_act(conv, m, act), want, rtol=1e-12, atol=1e-12)
+
+
+def test_layer_refusals():
+    from vfdepth_amd import kernels as KN
+    from vfdepth_amd import layers
+    with pytest.raises(ValueError, match='act is one of'):
+        layers.linear_act(torch.nn.Linear(2, 2), torch.zeros(1, 2), 'tanh')
+    for conv in (torch.nn.Conv2d(4, 4, 3), torch.nn.Conv2d(4, 4, 1, stride=2), torch.nn.Conv2d(4, 4, 1, groups=2),
+                 torch.nn.Conv2d(4, 4, 1, padding=1)):
+        with pytest.raises(ValueError, match='1x1'):
+            layers.linear_act(conv, torch.zeros(1, 4, 5, 5))
+    with pytest.raises(ValueError, match='1x1'):
+        layers.linear_act(torch.nn.Conv2d(4, 4, 1), torch.zeros(4, 5, 5))
+    with pytest.raises(RuntimeError, match='HIP device'):
+        KN.LinearAct.apply(torch.zeros(2, 3), torch.zeros(4, 3), None, None, 'none')
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+gpu = pytest.mark.gpu
+SHAPES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (5, 3, 7), (17, 64, 64), (6, 2048, 256), (33, 100, 31), (64, 96, 300), (65, 40, 513),
+          (128, 128, 128), (129, 127, 130), (256, 64, 256), (257, 1024, 96), (300, 517, 771), (1000, 8, 2000), (3000, 40, 24),
+          (520, 260, 260), (16, 4096, 512), (9000, 72, 136)]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', SHAPES)
+def test_shapes(M, K, N, dtype):
+    args = _case(M, K, N, dtype, seed=M + K)
+    _check(_run(*args, 'gelu'), *_oracle(*args, 'gelu'))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('bias,residual', [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize('act', ACTS)
+def test_activations(act, bias, residual, dtype):
+    args = _case(200, 96, 136, dtype, bias, residual, seed=len(act))
+    out = _run(*args, act)
+    _check(out, *_oracle(*args, act))
+    again = _run(*args, act)
+    assert all(torch.equal(a, b) for a, b in zip(out, again) if a is not None)
+    from vfdepth_amd import kernels as KN
+    with torch.no_grad():                                        # without a pre-activation to keep: the same bits
+        assert torch.equal(KN.LinearAct.apply(*args[:4], act), out[0])
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_large_product(dtype):
+    """Enough tiles for the largest tile form, ragged in each direction."""
+    args = _case(4200, 328, 4104, dtype, seed=7)
+    _check(_run(*args, 'silu'), *_oracle(*args, 'silu'))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_strides_offsets_and_leading_dimensions(dtype):
+    wide = torch.randn(60, 211, device='cuda').to(dtype)
+    w = (torch.randn(50, 100, device='cuda') * 0.1).to(dtype)
+    b = torch.randn(50, device='cuda').to(dtype)
+    for x in (wide[:, 8:108], wide[:, 3:103], wide[::2, 1:101], torch.randn(100, 60, device='cuda').to(dtype).t(),
+              torch.randn(100, device='cuda').to(dtype).expand(9, 100), wide.as_strided((20, 100), (7, 1))):
+        M = x.shape[0]
+        g = torch.randn(M, 50, device='cuda').to(dtype)
+        res = torch.randn(50, M, device='cuda').to(dtype).t()
+        args = [x.detach(), w, b, res.detach(), g]
+        _check(_run(*args, 'elu'), *_oracle(*args, 'elu'))
+    wt = (torch.randn(100, 50, device='cuda') * 0.1).to(dtype).t()              # a weight stored transposed
+    x = torch.randn(2, 3, 7, 100, device='cuda').to(dtype)
+    res = torch.randn(7, 50, device='cuda').to(dtype).expand(2, 3, 7, 50)
+    g = torch.randn(2, 3, 7, 50, device='cuda').to(dtype)
+    out = _run(x, wt, b, res.detach(), g, 'lrelu')
+    assert out[0].shape == g.shape and out[1].shape == x.shape
+    flat = lambda t: t.detach().reshape(-1, t.shape[-1])  # noqa: E731
+    vals, tol = _oracle(flat(x), wt, b, flat(res), flat(g), 'lrelu')
+    _check([flat(out[0]), flat(out[1]), out[2], out[3], flat(out[4])], vals, tol)
+    shared = torch.randn(1, 1, 1, 50, device='cuda').to(dtype).requires_grad_(True)          # a broadcast residual's gradient
+    from vfdepth_amd import kernels as KN
+    y = KN.LinearAct.apply(x, wt, b, shared.expand(2, 3, 7, 50), 'none')
+    ds, = torch.autograd.grad(y, shared, g)
+    want = g.cpu().double().sum((0, 1, 2))
+    lim = (HALF[dtype] + 50 * U) * g.cpu().double().abs().sum((0, 1, 2))
+    assert bool(((ds.flatten().cpu().double() - want).abs() <= lim).all())
+    s = KN.LinearAct.apply(x, wt, b, None, 'none').sum()                          # an expanded incoming gradient
+    s.backward()
+
+
+@gpu
+def test_no_rows():
+    from vfdepth_amd import kernels as KN
+    x = torch.empty(2, 0, 12, device='cuda', requires_grad=True)
+    w = torch.randn(5, 12, device='cuda', requires_grad=True)
+    b = torch.randn(5, device='cuda', requires_grad=True)
+    y = KN.LinearAct.apply(x, w, b, None, 'gelu')
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert y.shape == (2, 0, 5) and dx.shape == x.shape and not dw.any() and not db.any()
+
+
+@gpu
+@pytest.mark.parametrize('act', ['none', 'gelu'])
+def test_parts_of_the_gradient(act):
+    from vfdepth_amd import kernels as KN
+    x, w, b, res, g = _case(70, 48, 56, F32, seed=2)
+    vals, tol = _oracle(x, w, b, res, g, act)
+    for need in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 1, 0), (1, 0, 0, 1)):
+        leaves = [t.clone().requires_grad_(bool(n)) for t, n in zip((x, w, b, res), need)]
+        y = KN.LinearAct.apply(*leaves, act)
+        grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], g))
+        _check([y] + [next(grads) if n else None for n in need], vals, tol)
+
+
+@gpu
+def test_gradient_against_differences():
+    args = _case(20, 24, 28, F32, seed=5)
+    grads = _run(*args, 'gelu')[1:]
+    xs = [t.detach().cpu().double() for t in args[:4]]
+    gd = args[4].cpu().double()
+
+    def loss(x, w, b, res):
+        return float(((_slope(x @ w.t() + b, 'gelu')[0] + res) * gd).sum())
+    for k in range(4):
+        v = torch.randn(xs[k].shape, dtype=torch.float64, generator=torch.Generator().manual_seed(k))
+        up, dn = ([t + s * 1e-4 * v if i == k else t for i, t in enumerate(xs)] for s in (1, -1))
+        diff = (loss(*up) - loss(*dn)) / 2e-4
+        prod = grads[k].cpu().double() * v
+        assert abs(float(prod.sum()) - diff) <= 1e-5 * float(prod.abs().sum())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_non_finite_rows_stay_in_their_rows(dtype):
+    """Garbage in one row (or beyond the last) does not reach another: tiles are ragged in every direction here."""
+    from vfdepth_amd import kernels as KN
+    x, w, b, _, g = _case(150, 77, 90, dtype, seed=3)
+    with torch.no_grad():
+        good = KN.LinearAct.apply(x, w, b, None, 'relu')
+        wide = torch.full((152, 80), math.nan, device='cuda').to(dtype)
+        wide[1:151, 2:79] = x
+        wide[40, 5] = math.inf
+        y = KN.LinearAct.apply(wide[1:151, 2:79], w, b, None, 'relu')
+    keep = [i for i in range(150) if i != 39]
+    assert torch.equal(y[keep], good[keep]) and not torch.isfinite(y[39]).all()
+    xn = x.clone()
+    xn[3, 4] = math.nan
+    assert torch.isnan(KN.LinearAct.apply(xn, w, b, None, 'relu')[3]).all()
+
+
+@gpu
+def test_refusals():
+    from vfdepth_amd import kernels as KN
+    x, w, b, r, _ = _case(4, 8, 6, F32)
+    for args, word in (((x, w.to(BF16), None, None), 'weight'), ((x, w[:, :7], None, None), 'weight'),
+                       ((x, w, b[:5], None), 'bias'), ((x, w, b, r[:3]), 'residual'), ((x, w, b, r.to(BF16)), 'residual'),
+                       ((x.half(), w.half(), None, None), 'fp32 or bf16'), ((x, w.cpu(), None, None), 'HIP device'),
+                       ((x, w, b.cpu(), None), 'HIP device'), ((x, w.view(-1), None, None), 'weight'),
+                       ((x[:, :0], w[:, :0], None, None), 'at least 1'), ((x, w[:0], None, None), 'at least 1')):
+        with pytest.raises(RuntimeError, match=word):
+            KN.LinearAct.apply(*args, 'none')
+    with pytest.raises(ValueError, match='act is one of'):
+        KN.LinearAct.apply(x, w, b, r, 'softmax')
+    y = KN.LinearAct.apply(x.requires_grad_(True), w, b, r, 'gelu')
+    dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable|twice'):
+        dx.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize('fmt', [torch.channels_last, torch.contiguous_format])
+def test_conv_1x1(fmt):
+    from vfdepth_amd import layers
+    conv = torch.nn.Conv2d(40, 24, 1).cuda().to(memory_format=fmt)
+    x = torch.randn(2, 40, 5, 9, device='cuda').contiguous(memory_format=fmt).requires_grad_(True)
+    r = torch.randn(2, 24, 5, 9, device='cuda').contiguous(memory_format=fmt).requires_grad_(True)
+    g = torch.randn(2, 24, 5, 9, device='cuda')
+    y = layers.linear_act(conv, x, 'elu', r)
+    y.backward(g)
+    assert y.is_contiguous(memory_format=torch.channels_last) and conv.weight.grad.shape == (24, 40, 1, 1)
+    flat = lambda t: t.detach().permute(0, 2, 3, 1).reshape(-1, t.shape[1])  # noqa: E731
+    vals, tol = _oracle(flat(x), conv.weight.flatten(1), conv.bias, flat(r), flat(g), 'elu')
+    _check([flat(y), flat(x.grad), conv.weight.grad.flatten(1), conv.bias.grad, flat(r.grad)], vals, tol)
+
+
+@gpu
+def test_autocast():
+    """Under bf16 autocast the operands are cast once, and the fp32 parameters get fp32 gradients of the cast's."""
+    from vfdepth_amd import layers
+    lin = torch.nn.Linear(64, 72).cuda()
+    x, _, _, r, g = _case(90, 64, 72, BF16, seed=4)
+    x.requires_grad_(True)
+    with torch.autocast('cuda', dtype=BF16):
+        y = layers.linear_act(lin, x, 'gelu', r)
+    dx, dw, db = torch.autograd.grad(y, (x, lin.weight, lin.bias), g)
+    assert y.dtype == dx.dtype == BF16 and dw.dtype == db.dtype == F32
+    vals, tol = _oracle(x, lin.weight.to(BF16), lin.bias.to(BF16), r, g, 'gelu')
+    _check([y, dx, dw.to(BF16), db.to(BF16)], vals, tol)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_streams_and_captured_graph(dtype):
+    from vfdepth_amd import kernels as KN
+    args = _case(3000, 40, 24, dtype, seed=9)                        # the weight's gradient is split and joined
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = _run(*args, 'silu')
+    torch.cuda.current_stream().wait_stream(side)
+    _check(out, *_oracle(*args, 'silu'))
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _run(*args, 'silu')
+    out = [t.detach() for t in out]
+    for k in range(4):
+        with torch.no_grad():
+            for t, s in zip(args, _case(3000, 40, 24, dtype, seed=30 + k)):
+                t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, *_oracle(*args, 'silu'))
+        with torch.no_grad():
+            assert torch.equal(KN.LinearAct.apply(*args[:4], 'silu'), out[0])         # eager work between replays

@@ -52,6 +52,18 @@ class BnDesc(ctypes.Structure):
                 ('nhwc', c_int), ('groups', c_int)]
 
 
+class NormDesc(ctypes.Structure):
+    _fields_ = [('rows', c_int), ('cols', c_int), ('ldx', ctypes.c_int64), ('eps', c_float), ('dtype', c_int)]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [('rows', c_int), ('k', c_int), ('n', c_int), ('act', c_int), ('ldx', ctypes.c_int64), ('dtype', c_int)]
+
+
+# vfd_linear_workspace's calls and vfd_linear_desc.act
+LINEAR_FWD, LINEAR_DGRAD, LINEAR_WGRAD, LINEAR_ACT_BWD = range(4)
+LINEAR_ACTS = {'none': 0, 'relu': 1, 'lrelu': 2, 'elu': 3, 'gelu': 4, 'silu': 5}
+
 _SIGS = {
     'vfd_version': (c_int, []),
     'vfd_last_error': (ctypes.c_char_p, []),
@@ -159,6 +171,17 @@ _SIGS = {
     'vfd_depth_syn_bwd': (c_int, [ctypes.POINTER(DepthSynDesc)] + [c_fp] * 9 + [c_void_p]),
     'vfd_depth_syn_bwd_ordered_workspace': (ctypes.c_size_t, [ctypes.POINTER(DepthSynDesc)]),
     'vfd_depth_syn_bwd_ordered': (c_int, [ctypes.POINTER(DepthSynDesc)] + [c_fp] * 10 + [ctypes.c_size_t, c_void_p]),
+    'vfd_layer_norm_fwd': (c_int, [ctypes.POINTER(NormDesc)] + [c_fp] * 6 + [c_void_p]),
+    'vfd_layer_norm_bwd_workspace': (c_size_t, [ctypes.POINTER(NormDesc)]),
+    'vfd_layer_norm_bwd': (c_int, [ctypes.POINTER(NormDesc)] + [c_fp] * 9 + [c_size_t, c_void_p]),
+    'vfd_linear_workspace': (c_size_t, [ctypes.POINTER(LinearDesc), c_int]),
+    'vfd_linear_fwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 7 + [c_size_t, c_void_p]),
+    'vfd_linear_act_bwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 5 + [c_size_t, c_void_p]),
+    'vfd_linear_dgrad': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 4 + [c_size_t, c_void_p]),
+    'vfd_linear_wgrad': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 4 + [c_size_t, c_void_p]),
+    'vfd_grad_norm_workspace': (c_size_t, [c_int, c_fp]),
+    'vfd_grad_norm': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_fp, c_fp, c_size_t, c_void_p]),
+    'vfd_clip_grads': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_double] + [c_fp] * 4 + [c_size_t, c_void_p]),
     'vfd_smooth_workspace_bytes': (c_size_t, [c_int] * 4),
     'vfd_smooth_fwd': (c_int, [c_int] * 4 + [c_fp] * 5 + [c_size_t, c_void_p]),
     'vfd_smooth_bwd': (c_int, [c_int] * 4 + [c_fp] * 5 + [c_void_p]),
@@ -207,7 +230,8 @@ KERNEL_IDS = {
     'voxel_project_fwd': 5, 'voxel_project_bwd': 6, 'view_stats': 7, 'view_apply': 8, 'view_bwd': 9,
     'photo_fwd': 10, 'photo_bwd': 11, 'smooth_fwd': 12, 'smooth_bwd': 13, 'fusion_plan': 14,
     'aggregate': 15, 'voxel_project_plan': 16, 'proj_conv_fwd': 17,
-    'depth_syn_fwd': 18, 'depth_syn_bwd': 19, 'proj_conv_dgrad': 20, 'pad_conv_fwd': 21, 'bn_fwd': 22, 'bn_bwd': 23, 'reflect_pad': 24, 'upsample_bwd': 25, 'maxpool': 26, 'elu_pad': 27, 'disp_conv': 28, 'dec_conv': 29, 'proj_conv_wgrad': 30, 'pad_conv_dgrad': 31, 'pad_conv_wgrad': 32, 'layout_copy': 33,
+    'depth_syn_fwd': 18, 'depth_syn_bwd': 19, 'proj_conv_dgrad': 20, 'pad_conv_fwd': 21, 'bn_fwd': 22, 'bn_bwd': 23, 'reflect_pad': 24, 'upsample_bwd': 25, 'maxpool': 26, 'elu_pad': 27, 'disp_conv': 28, 'dec_conv': 29, 'proj_conv_wgrad': 30, 'pad_conv_dgrad': 31, 'pad_conv_wgrad': 32, 'layout_copy': 33, 'grad_clip': 34, 'layer_norm_fwd': 35, 'layer_norm_bwd': 36,
+    'linear_fwd': 37, 'linear_bwd': 38,
 }
 
 
@@ -230,7 +254,8 @@ def prof_enable(kernel='all'):
 # Algorithmic bytes of the shape-varying dense-net kernels (fused BN, reflect pads, upsample
 # backward), accumulated by their Python wrappers while profiling is on (bench.py's rooflines).
 PROF_ON = False
-ALG_BYTES = {'bn_fwd': 0, 'bn_bwd': 0, 'reflect_pad': 0, 'upsample_bwd': 0, 'maxpool': 0, 'elu_pad': 0, 'disp_conv': 0, 'dec_conv': 0, 'layout_copy': 0}
+ALG_BYTES = {'bn_fwd': 0, 'bn_bwd': 0, 'reflect_pad': 0, 'upsample_bwd': 0, 'maxpool': 0, 'elu_pad': 0, 'disp_conv': 0, 'dec_conv': 0, 'layout_copy': 0,
+             'grad_clip': 0, 'layer_norm_fwd': 0, 'layer_norm_bwd': 0, 'linear_fwd': 0, 'linear_bwd': 0}
 
 
 def prof_read():

@@ -107,6 +107,8 @@ def surround_fusion_cfg(**over):
             # build-only: precision of the dense nets (encoders/decoders/reduce_dim on MIOpen);
             # 'bf16' = autocast for config 3, the HIP fusion/geometry/loss kernels stay fp32
             'net_precision': 'fp32',
+            # build-only: global gradient norm to clip to before each optimizer step (0: no clipping)
+            'max_grad_norm': 0.0,
         },
         'loss': {'disparity_smoothness': 0.001, 'spatio_coeff': 0.03,
                  'spatio_tempo_coeff': 0.1, 'pose_loss_coeff': 0.0},

@@ -1,0 +1,532 @@
+// Matrix product with bias, activation and residual in its epilogue (a linear layer, or a 1x1 convolution of a
+// channels-last map), forward and backward, on the matrix cores:
+//   z = x W^T + b,   y = act(z) + r            x [M, K], W [N, K], y, z, r [M, N]
+//   gz = g act'(z),  d x = gz W,  d W = gz^T x,  d b = column sums of gz,  d r = g
+// fp32 (v_mfma_f32_32x32x2_f32) or bf16 (v_mfma_f32_32x32x16_bf16, fp32 sums, each output rounded once).
+//
+// One tile kernel serves the three products: an operand is read as [outer][contraction] (its contraction contiguous:
+// x, W and gz forward) or as [contraction][outer] (W and gz, x in the gradients), and leaves LDS in the matrix
+// instructions' order either way, so nothing is transposed in memory.
+#include <type_traits>
+
+#include "vfd_common.h"
+
+namespace vfd {
+
+typedef float lin_f16 __attribute__((ext_vector_type(16)));
+typedef float lin_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 lin_b8 __attribute__((ext_vector_type(8)));
+typedef short lin_s4 __attribute__((ext_vector_type(4)));
+
+enum LinAct { LIN_NONE = 0, LIN_RELU, LIN_LRELU, LIN_ELU, LIN_GELU, LIN_SILU, LIN_ACTS };
+constexpr float LIN_SLOPE = 0.1f;            // the framework's LeakyReLU
+
+template <int ACT>
+__device__ __forceinline__ float lin_act(float z) {
+  if constexpr (ACT == LIN_RELU) return z <= 0.f ? 0.f : z;               // NaN passes
+  if constexpr (ACT == LIN_LRELU) return z > 0.f ? z : LIN_SLOPE * z;
+  if constexpr (ACT == LIN_ELU) return z > 0.f ? z : expm1f(z);
+  if constexpr (ACT == LIN_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == LIN_SILU) return z / (1.f + expf(-z));
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float lin_slope(float z) {
+  if constexpr (ACT == LIN_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == LIN_LRELU) return z > 0.f ? 1.f : LIN_SLOPE;
+  if constexpr (ACT == LIN_ELU) return z > 0.f ? 1.f : expf(z);
+  if constexpr (ACT == LIN_GELU)
+    return fmaf(z, expf(-0.5f * z * z) * 0.39894228040143268f, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if constexpr (ACT == LIN_SILU) {
+    const float s = 1.f / (1.f + expf(-z));
+    return s * fmaf(z, 1.f - s, 1.f);
+  }
+  return 1.f;
+}
+
+template <typename F>
+static int lin_with_act(int act, F f) {
+  switch (act) {
+    case LIN_RELU: return f(std::integral_constant<int, LIN_RELU>());
+    case LIN_LRELU: return f(std::integral_constant<int, LIN_LRELU>());
+    case LIN_ELU: return f(std::integral_constant<int, LIN_ELU>());
+    case LIN_GELU: return f(std::integral_constant<int, LIN_GELU>());
+    case LIN_SILU: return f(std::integral_constant<int, LIN_SILU>());
+    default: return f(std::integral_constant<int, LIN_NONE>());
+  }
+}
+
+// ---------------------------------------------------------------- tile kernel
+template <typename T>
+struct LinT {
+  static constexpr int VE = 16 / (int)sizeof(T);        // values of a 16-byte chunk
+  static constexpr int BK = 128 / (int)sizeof(T);       // contraction values of a staged tile
+  typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+  typedef T avec __attribute__((ext_vector_type(16 / sizeof(T))));
+};
+
+__device__ __forceinline__ lin_f16 lin_mma(lin_b8 a, lin_b8 b, lin_f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// four steps of two contraction values: lane halves hold values 4 h + j of each group of eight
+__device__ __forceinline__ lin_f16 lin_mma(lin_f4 a, lin_f4 b, lin_f16 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// One operand of a product: element (o, k) at p[o * ld + k] (MC = false) or p[k * ld + o] (MC = true).
+template <typename T>
+struct LinOp {
+  const T* p;
+  long long ld;
+  int O, K;
+};
+
+// A tile of BO outer by BK contraction values in LDS, BO * 128 bytes.
+//   MC = false: rows of 128 bytes, one per outer index; 16-byte chunk c of row o lies at chunk c ^ (o & 7), so that the
+//     8 rows a group of lanes reads at one chunk fall on 8 different bank groups.
+//   MC = true: rows of BO values, one per contraction index, 32-byte pairs of chunks exchanged by (k & 3) (bf16: the
+//     transposing read takes 4 rows at once; fp32 lanes read consecutive values).
+template <typename T, bool MC, int BO, int NT>
+struct LinTile {
+  typedef LinT<T> X;
+  static constexpr int NCH = BO * 8 / NT;               // chunks a thread stages
+  static constexpr int CPR = BO / X::VE;                // chunks of a contraction row
+  static_assert(BO * 8 % NT == 0, "whole chunks a thread");
+
+  static __device__ __forceinline__ int at(int row, int c) {       // byte offset of a chunk
+    if constexpr (!MC) return row * 128 + ((c ^ (row & 7)) << 4);
+    return row * (BO * (int)sizeof(T)) + ((sizeof(T) == 2 ? (c ^ ((row & 3) << 1)) : c) << 4);
+  }
+  static __device__ __forceinline__ void fetch(const LinOp<T>& op, int o0, int k0, typename X::vec (&v)[NCH]) {
+    const bool whole = o0 + BO <= op.O && k0 + X::BK <= op.K;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int e = (int)threadIdx.x + i * NT;
+      const int row = MC ? e / CPR : e >> 3, c = MC ? e % CPR : e & 7;
+      const int o = o0 + (MC ? c * X::VE : row), k = k0 + (MC ? row : c * X::VE);
+      const T* p = op.p + (MC ? (size_t)k * op.ld + o : (size_t)o * op.ld + k);
+      if (whole) {
+        v[i] = *reinterpret_cast<const typename X::vec*>(p);
+      } else {
+        const int n = (o < op.O && k < op.K) ? min(MC ? op.O - o : op.K - k, X::VE) : 0;
+        if (n == X::VE) {
+          v[i] = *reinterpret_cast<const typename X::vec*>(p);
+        } else {
+#pragma unroll
+          for (int j = 0; j < X::VE; ++j) v[i][j] = (T)0.f;
+#pragma unroll
+          for (int j = 0; j < X::VE; ++j)
+            if (j < n) v[i][j] = p[j];
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void put(char* lds, const typename X::vec (&v)[NCH]) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int e = (int)threadIdx.x + i * NT;
+      *reinterpret_cast<typename X::avec*>(lds + (MC ? at(e / CPR, e % CPR) : at(e >> 3, e & 7))) = v[i];
+    }
+  }
+  // The 32 outer indices from o on, contraction step ks (of 4): lane l holds outer l & 31, 16 bytes of contraction
+  static __device__ __forceinline__ typename X::avec frag(const char* lds, int o, int ks) {
+    const int lane = threadIdx.x & 63;
+    typename X::avec r;
+    if constexpr (!MC) {
+      r = *reinterpret_cast<const typename X::avec*>(lds + at(o + (lane & 31), 2 * ks + (lane >> 5)));
+    } else if constexpr (sizeof(T) == 2) {
+      // transposing read: lane 4 q + p of 16-lane group gq supplies row q, columns 4 p .. of column half gq & 1
+      const int gq = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+      const int col = o + 16 * (gq & 1) + 4 * p, k = 16 * ks + 8 * (gq >> 1) + q;
+      typedef __attribute__((address_space(3))) lin_s4 lds_s4;
+      const lin_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + at(k, col >> 3) + (col & 7) * 2));
+      const lin_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds + at(k + 4, col >> 3) + (col & 7) * 2));
+      __builtin_memcpy(&r, &a, 8);
+      __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &b, 8);
+    } else {
+      const int k = 8 * ks + 4 * (lane >> 5);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(lds + (k + j) * (BO * 4) + (o + (lane & 31)) * 4);
+    }
+    return r;
+  }
+};
+
+template <typename T>
+struct LinEpi {
+  const T* bias;                 // [N], null
+  const T* res;                  // [M, N], null
+  T* z;                          // [M, N], null: pre-activation for the backward
+  T* y;                          // [M, N]
+  float* part;                   // [splits, M, N] where the contraction is split (then nothing else is used)
+  int act;
+};
+
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep, int tm, int tn, int splits) {
+  constexpr int NT = 64 * WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+  typedef LinT<T> X;
+  typedef LinTile<T, XMC, BM, NT> TX;
+  typedef LinTile<T, WMC, BN, NT> TW;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int STAGE = (BM + BN) * 128;
+  // tiles of one XCD (every eighth workgroup) are consecutive: column groups of 8 row tiles, splits outermost
+  const int total = tm * tn * splits, xcd = blockIdx.x % 8, per = total / 8, rest = total % 8;
+  int t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
+  const int split = t / (tm * tn);
+  t -= split * tm * tn;
+  constexpr int GM = 8;
+  const int group = t / (GM * tn), g0 = group * GM, gm = min(GM, tm - g0);
+  t -= group * GM * tn;
+  const int m0 = (g0 + t % gm) * BM, n0 = (t / gm) * BN;
+  const int kt = (x.K + X::BK - 1) / X::BK;
+  const int k_lo = (int)((long long)kt * split / splits), k_hi = (int)((long long)kt * (split + 1) / splits);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = (wave % WM) * FM * 32, wn = (wave / WM) * FN * 32;
+
+  lin_f16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  typename X::vec vx[TX::NCH], vw[TW::NCH];
+  if (k_lo < k_hi) {
+    TX::fetch(x, m0, k_lo * X::BK, vx);
+    TW::fetch(w, n0, k_lo * X::BK, vw);
+    TX::put(lds, vx);
+    TW::put(lds + BM * 128, vw);
+  }
+  __syncthreads();
+  for (int k = k_lo; k < k_hi; ++k) {
+    const char* cur = lds + ((k - k_lo) & 1) * STAGE;
+    char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
+    if (k + 1 < k_hi) {
+      TX::fetch(x, m0, (k + 1) * X::BK, vx);
+      TW::fetch(w, n0, (k + 1) * X::BK, vw);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      typename X::avec fx[FM], fw[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[i] = TX::frag(cur, wm + 32 * i, ks);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fw[j] = TW::frag(cur + BM * 128, wn + 32 * j, ks);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = lin_mma(fw[j], fx[i], acc[i][j]);
+    }
+    if (k + 1 < k_hi) {
+      TX::put(nxt, vx);
+      TW::put(nxt + BM * 128, vw);
+    }
+    __syncthreads();
+  }
+
+  // D of a block: column (lane & 31) = row of y, 4 consecutive columns of y per group of 4 registers
+  const int M = x.O, N = w.O;
+  auto with_act = [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = m0 + wm + 32 * i + (lane & 31);
+      if (m >= M) continue;
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + wn + 32 * j + 8 * q + 4 * (lane >> 5);
+          const size_t at = (size_t)m * N + n;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (n + e >= N) continue;
+            float v = acc[i][j][4 * q + e];
+            if constexpr (decltype(act)::value < 0) {
+              ep.part[(size_t)split * M * N + at + e] = v;
+            } else {
+              if (ep.bias) v += ld1(ep.bias + n + e);
+              if (ep.z) st1(ep.z + at + e, v);
+              v = lin_act<decltype(act)::value>(v);
+              if (ep.res) v += ld1(ep.res + at + e);
+              st1(ep.y + at + e, v);
+            }
+          }
+        }
+    }
+  };
+  if (ep.part) {
+    with_act(std::integral_constant<int, -1>());
+    return;
+  }
+  switch (ep.act) {
+    case LIN_RELU: with_act(std::integral_constant<int, LIN_RELU>()); break;
+    case LIN_LRELU: with_act(std::integral_constant<int, LIN_LRELU>()); break;
+    case LIN_ELU: with_act(std::integral_constant<int, LIN_ELU>()); break;
+    case LIN_GELU: with_act(std::integral_constant<int, LIN_GELU>()); break;
+    case LIN_SILU: with_act(std::integral_constant<int, LIN_SILU>()); break;
+    default: with_act(std::integral_constant<int, LIN_NONE>()); break;
+  }
+}
+
+// A split contraction's partial products, added in split order, and the epilogue.
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, size_t mn, int N) {
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < mn; i += (size_t)gridDim.x * 1024) {
+    float v[4];
+    const int c = mn - i < 4 ? (int)(mn - i) : 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 0.f;
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < c) v[e] += ep.part[(size_t)s * mn + i + e];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= c) continue;
+      if (ep.bias) v[e] += ld1(ep.bias + (i + e) % N);
+      if (ep.z) st1(ep.z + i + e, v[e]);
+      v[e] = lin_act<ACT>(v[e]);
+      if (ep.res) v[e] += ld1(ep.res + i + e);
+      st1(ep.y + i + e, v[e]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gz = g act'(z) and its column sums
+// A block owns `cols` = 64 V columns of a strip of rows, four rows at a time (one per wave): gz written as it is read,
+// the columns' sums kept in registers and left as one partial row per block (added in block order by col_sums_k).
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, const T* __restrict__ z, T* __restrict__ gz,
+                                                     float* __restrict__ part, int M, int N) {
+  constexpr int V = LinT<T>::VE;
+  typedef typename LinT<T>::vec vec;
+  __shared__ float sm[4][64][V + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = (blockIdx.x * 64 + lane) * V, cnt = min(max(N - n, 0), V);
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = 0.f;
+  if (cnt > 0)
+    for (long long m = (long long)blockIdx.y * 4 + wave; m < M; m += (long long)gridDim.y * 4) {
+      const size_t at = (size_t)m * N + n;
+      vec gv, zv, o;
+      if (cnt == V) {
+        gv = *reinterpret_cast<const vec*>(g + at);
+        if (ACT != LIN_NONE) zv = *reinterpret_cast<const vec*>(z + at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          gv[j] = j < cnt ? g[at + j] : (T)0.f;
+          if (ACT != LIN_NONE) zv[j] = j < cnt ? z[at + j] : (T)0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float f = (float)gv[j];
+        if (ACT != LIN_NONE) f *= lin_slope<ACT>((float)zv[j]);
+        s[j] += f;
+        o[j] = (T)f;
+      }
+      if (ACT != LIN_NONE) {
+        if (cnt == V) {
+          *reinterpret_cast<vec*>(gz + at) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j < cnt) gz[at + j] = o[j];
+        }
+      }
+    }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) sm[wave][lane][j] = s[j];
+  __syncthreads();
+  if (wave == 0)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < cnt)
+        part[(size_t)blockIdx.y * N + n + j] = (sm[0][lane][j] + sm[1][lane][j]) + (sm[2][lane][j] + sm[3][lane][j]);
+}
+
+// ---------------------------------------------------------------- host
+constexpr int LIN_CUS = 256;
+
+struct LinPlan {
+  int tm, tn, splits;
+};
+
+// Tiles of BM x BN, and how often the contraction is split so that a product with few tiles still fills the chip (a
+// split keeps at least four staged tiles of work).
+template <typename T, int BM, int BN>
+static LinPlan lin_plan(int M, int N, int K, int resident) {
+  LinPlan p;
+  p.tm = (M + BM - 1) / BM;
+  p.tn = (N + BN - 1) / BN;
+  const long long tiles = (long long)p.tm * p.tn, kt = (K + LinT<T>::BK - 1) / LinT<T>::BK;
+  long long s = (long long)LIN_CUS * resident / tiles;
+  if (s > kt / 4) s = kt / 4;
+  p.splits = s < 1 ? 1 : (int)s;
+  return p;
+}
+
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN>
+static int lin_launch(const LinOp<T>& x, const LinOp<T>& w, LinEpi<T> ep, const LinPlan& p, float* part, hipStream_t s) {
+  auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN>;
+  constexpr int bytes = 2 * (BM + BN) * 128;
+  lds_attr((const void*)fn, bytes);
+  ep.part = p.splits > 1 ? part : nullptr;
+  fn<<<(unsigned)(p.tm * p.tn * p.splits), 64 * WM * WN, bytes, s>>>(x, w, ep, p.tm, p.tn, p.splits);
+  if (p.splits > 1) {
+    const size_t mn = (size_t)x.O * w.O;
+    const size_t blocks = (mn + 1023) / 1024;
+    lin_with_act(ep.act, [&](auto act) {
+      lin_join_k<T, act()><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, mn, w.O);
+      return 0;
+    });
+  }
+  return fail_launch("linear");
+}
+
+constexpr int LIN_BM = 128, LIN_BN = 128, LIN_RES = 2;
+
+template <typename T, bool XMC, bool WMC>
+static int lin_product(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, float* part, hipStream_t s) {
+  return lin_launch<T, XMC, WMC, LIN_BM, LIN_BN, 2, 2>(x, w, ep, lin_plan<T, LIN_BM, LIN_BN>(x.O, w.O, x.K, LIN_RES), part, s);
+}
+
+template <typename T>
+static size_t lin_part_bytes(int M, int N, int K) {
+  const LinPlan p = lin_plan<T, LIN_BM, LIN_BN>(M, N, K, LIN_RES);
+  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+}
+
+static int lin_strips(int M, int N, int V) {               // row blocks of lin_act_bwd_k
+  const int cb = (N + 64 * V - 1) / (64 * V), most = 2048 / cb > 0 ? 2048 / cb : 1, need = (M + 15) / 16;
+  return need < most ? need : most;
+}
+
+template <typename T>
+static size_t lin_ws(const vfd_linear_desc* d, int what) {
+  switch (what) {
+    case VFD_LINEAR_FWD: return lin_part_bytes<T>(d->rows, d->n, d->k);
+    case VFD_LINEAR_DGRAD: return lin_part_bytes<T>(d->rows, d->k, d->n);
+    case VFD_LINEAR_WGRAD: return lin_part_bytes<T>(d->n, d->k, d->rows);
+    case VFD_LINEAR_ACT_BWD: return (size_t)lin_strips(d->rows, d->n, LinT<T>::VE) * d->n * sizeof(float);
+  }
+  return 0;
+}
+
+static int lin_check(const char* what, const vfd_linear_desc* d) {
+  VFD_REQUIRE(d && d->rows >= 0 && d->k >= 0 && d->n >= 0 && d->rows <= VFD_LINEAR_MAX && d->k <= VFD_LINEAR_MAX &&
+                  d->n <= VFD_LINEAR_MAX && d->ldx >= d->k && d->act >= 0 && d->act < LIN_ACTS && (d->dtype == 0 || d->dtype == 1),
+              "%s: bad descriptor", what);
+  const long long T = 128;
+  VFD_REQUIRE(((long long)d->rows / T + 1) * (d->n / T + 1) < (1 << 30) && ((long long)d->rows / T + 1) * (d->k / T + 1) < (1 << 30) &&
+                  ((long long)d->n / T + 1) * (d->k / T + 1) < (1 << 30),
+              "%s: too many tiles", what);
+  return VFD_OK;
+}
+
+template <typename T>
+static int lin_fwd_run(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y,
+                       void* z, float* part, hipStream_t s) {
+  const LinOp<T> ox{(const T*)x, d->ldx, d->rows, d->k}, ow{(const T*)w, d->k, d->n, d->k};
+  const LinEpi<T> ep{(const T*)bias, (const T*)res, (T*)z, (T*)y, nullptr, d->act};
+  return lin_product<T, false, false>(ox, ow, ep, part, s);
+}
+
+template <typename T>
+static int lin_dgrad_run(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, float* part, hipStream_t s) {
+  const LinOp<T> og{(const T*)gz, d->n, d->rows, d->n}, ow{(const T*)w, d->k, d->k, d->n};
+  const LinEpi<T> ep{nullptr, nullptr, nullptr, (T*)dx, nullptr, LIN_NONE};
+  return lin_product<T, false, true>(og, ow, ep, part, s);
+}
+
+template <typename T>
+static int lin_wgrad_run(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, float* part, hipStream_t s) {
+  const LinOp<T> og{(const T*)gz, d->n, d->n, d->rows}, ox{(const T*)x, d->ldx, d->k, d->rows};
+  const LinEpi<T> ep{nullptr, nullptr, nullptr, (T*)dw, nullptr, LIN_NONE};
+  return lin_product<T, true, true>(og, ox, ep, part, s);
+}
+
+template <typename T>
+static int lin_act_bwd_run(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, float* part, hipStream_t s) {
+  const int strips = lin_strips(d->rows, d->n, LinT<T>::VE);
+  const dim3 grid(cdiv(d->n, 64 * LinT<T>::VE), strips);
+  lin_with_act(d->act, [&](auto act) {
+    lin_act_bwd_k<T, act()><<<grid, 256, 0, s>>>((const T*)g, (const T*)z, (T*)gz, db ? part : nullptr, d->rows, d->n);
+    return 0;
+  });
+  if (db) col_sums_k<T><<<cdiv(d->n, COLSUM_COLS), 1024, 0, s>>>(part, strips, d->n, d->n, (T*)db, nullptr);
+  return fail_launch("linear_act_bwd");
+}
+
+}  // namespace vfd
+
+using namespace vfd;
+
+extern "C" {
+
+size_t vfd_linear_workspace(const vfd_linear_desc* d, int what) {
+  if (lin_check("linear", d) != VFD_OK || d->rows == 0 || d->k == 0 || d->n == 0) return 0;
+  return d->dtype ? lin_ws<__bf16>(d, what) : lin_ws<float>(d, what);
+}
+
+int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z,
+                   void* workspace, size_t ws_bytes, void* stream) {
+  if (int e = lin_check("linear_fwd", d)) return e;
+  if (d->rows == 0 || d->n == 0) return VFD_OK;
+  VFD_REQUIRE(y && (d->k == 0 || (x && w)), "linear_fwd: null tensor");
+  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_FWD);
+  VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_fwd: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  ProfScope prof(K_LINEAR_FWD, s);
+  return (d->dtype ? lin_fwd_run<__bf16> : lin_fwd_run<float>)(d, x, w, bias, res, y, z, (float*)workspace, s);
+}
+
+int vfd_linear_act_bwd(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, void* workspace,
+                       size_t ws_bytes, void* stream) {
+  if (int e = lin_check("linear_act_bwd", d)) return e;
+  hipStream_t s = (hipStream_t)stream;
+  ProfScope prof(K_LINEAR_BWD, s);
+  if (d->n == 0) return VFD_OK;
+  if (d->rows == 0) {
+    if (db) zero_async(db, (size_t)d->n * (d->dtype ? 2 : 4), s);
+    return fail_launch("linear_act_bwd");
+  }
+  VFD_REQUIRE(g && (d->act == LIN_NONE || (z && gz)), "linear_act_bwd: null tensor");
+  if (d->act == LIN_NONE && !db) return VFD_OK;
+  const size_t need = (size_t)lin_strips(d->rows, d->n, d->dtype ? 8 : 4) * d->n * sizeof(float);
+  VFD_REQUIRE(!db || (workspace && ws_bytes >= need), "linear_act_bwd: workspace too small");
+  return (d->dtype ? lin_act_bwd_run<__bf16> : lin_act_bwd_run<float>)(d, g, z, gz, db, (float*)workspace, s);
+}
+
+int vfd_linear_dgrad(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, void* workspace, size_t ws_bytes,
+                     void* stream) {
+  if (int e = lin_check("linear_dgrad", d)) return e;
+  if (d->rows == 0 || d->k == 0) return VFD_OK;
+  VFD_REQUIRE(dx && (d->n == 0 || (gz && w)), "linear_dgrad: null tensor");
+  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_DGRAD);
+  VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_dgrad: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  ProfScope prof(K_LINEAR_BWD, s);
+  return (d->dtype ? lin_dgrad_run<__bf16> : lin_dgrad_run<float>)(d, gz, w, dx, (float*)workspace, s);
+}
+
+int vfd_linear_wgrad(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, void* workspace, size_t ws_bytes,
+                     void* stream) {
+  if (int e = lin_check("linear_wgrad", d)) return e;
+  if (d->k == 0 || d->n == 0) return VFD_OK;
+  VFD_REQUIRE(dw && (d->rows == 0 || (gz && x)), "linear_wgrad: null tensor");
+  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_WGRAD);
+  VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_wgrad: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  ProfScope prof(K_LINEAR_BWD, s);
+  return (d->dtype ? lin_wgrad_run<__bf16> : lin_wgrad_run<float>)(d, gz, x, dw, (float*)workspace, s);
+}
+
+}  // extern "C"

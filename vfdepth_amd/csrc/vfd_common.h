@@ -30,7 +30,8 @@ void lds_attr(const void* fn, int bytes);
 enum KernelId {
   K_MASK_DOWN = 0, K_FUSE_DEPTH_FWD, K_FUSE_DEPTH_BWD, K_FUSE_POSE_FWD, K_FUSE_POSE_BWD,
   K_VPROJ_FWD, K_VPROJ_BWD, K_VIEW_STATS, K_VIEW_APPLY, K_VIEW_BWD, K_PHOTO_FWD, K_PHOTO_BWD,
-  K_SMOOTH_FWD, K_SMOOTH_BWD, K_FUSION_PLAN, K_AGGREGATE, K_VPROJ_PLAN, K_PROJ_CONV_FWD, K_DEPTH_SYN_FWD, K_DEPTH_SYN_BWD, K_PROJ_CONV_DGRAD, K_PAD_CONV_FWD, K_BN_FWD, K_BN_BWD, K_REFLECT_PAD, K_UPSAMPLE_BWD, K_MAXPOOL, K_ELU_PAD, K_DISP_CONV, K_DEC_CONV, K_PROJ_CONV_WGRAD, K_PAD_CONV_DGRAD, K_PAD_CONV_WGRAD, K_LAYOUT_COPY, K_COUNT
+  K_SMOOTH_FWD, K_SMOOTH_BWD, K_FUSION_PLAN, K_AGGREGATE, K_VPROJ_PLAN, K_PROJ_CONV_FWD, K_DEPTH_SYN_FWD, K_DEPTH_SYN_BWD, K_PROJ_CONV_DGRAD, K_PAD_CONV_FWD, K_BN_FWD, K_BN_BWD, K_REFLECT_PAD, K_UPSAMPLE_BWD, K_MAXPOOL, K_ELU_PAD, K_DISP_CONV, K_DEC_CONV, K_PROJ_CONV_WGRAD, K_PAD_CONV_DGRAD, K_PAD_CONV_WGRAD, K_LAYOUT_COPY,
+  K_GRAD_CLIP, K_LN_FWD, K_LN_BWD, K_LINEAR_FWD, K_LINEAR_BWD, K_COUNT
 };
 void prof_begin(int id, hipStream_t s);
 void prof_end(int id, hipStream_t s);
@@ -290,6 +291,40 @@ static inline void zero_async(void* p, size_t bytes, hipStream_t s) {
   size_t blocks = (bytes / 16 + 255) / 256;
   blocks = blocks < 1 ? 1 : (blocks > 2048 ? 2048 : blocks);
   zero_fill_k<<<(unsigned)blocks, 256, 0, s>>>((unsigned char*)p, bytes);
+}
+
+// Column sums of partial rows [nb][n] in row order: columns 0 .. split - 1 into a, the others into b (either may be
+// null).  64 slices of the rows a column: with one thread a column, 1024 dependent rounds of latency were the whole time.
+constexpr int COLSUM_COLS = 16;
+template <typename O>
+__global__ __launch_bounds__(1024) void col_sums_k(const float* __restrict__ part, int nb, int n, int split,
+                                                   O* __restrict__ a, O* __restrict__ b) {
+  __shared__ float sm[64][COLSUM_COLS + 1];
+  const int lc = threadIdx.x % COLSUM_COLS, sl = threadIdx.x / COLSUM_COLS;
+  const size_t c = (size_t)blockIdx.x * COLSUM_COLS + lc;
+  float s = 0.f;
+  if (c < (size_t)n) {
+    int k = sl;
+    for (; k + 192 < nb; k += 256) {
+      const float v0 = part[(size_t)k * n + c], v1 = part[(size_t)(k + 64) * n + c], v2 = part[(size_t)(k + 128) * n + c],
+                  v3 = part[(size_t)(k + 192) * n + c];
+      s += (v0 + v1) + (v2 + v3);
+    }
+    for (; k < nb; k += 64) s += part[(size_t)k * n + c];
+  }
+  sm[sl][lc] = s;
+  __syncthreads();
+  for (int h = 32; h > 0; h >>= 1) {
+    if (sl < h) sm[sl][lc] += sm[sl + h][lc];
+    __syncthreads();
+  }
+  if (sl == 0 && c < (size_t)n) {
+    if (c < (size_t)split) {
+      if (a != nullptr) st1(a + c, sm[0][lc]);
+    } else if (b != nullptr) {
+      st1(b + (c - split), sm[0][lc]);
+    }
+  }
 }
 
 }  // namespace vfd

@@ -4,6 +4,7 @@ Each op is a `torch.autograd.Function` whose forward and backward are single C-A
 current HIP stream.  Inputs must be fp32 HIP tensors; there is no CPU or ATen fallback — a
 missing library or a non-HIP tensor raises.
 """
+import array
 import ctypes
 import math
 import os
@@ -11,6 +12,7 @@ import weakref
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -2114,3 +2116,271 @@ class MaxPool3s2(torch.autograd.Function):
         if L.PROF_ON:
             L.ALG_BYTES['maxpool'] += (g.numel() + dx.numel()) * dx.element_size() + arg.numel()
         return dx
+
+
+# =============================================================================================
+# Layer norm over the last dimension
+# =============================================================================================
+def _rows(x, what):
+    """x [..., C] as (rows [R, C] with a unit last stride, elements from one row to the next): a view where x's
+    leading dimensions are evenly spaced, a copy otherwise."""
+    C = x.shape[-1]
+    x2 = x.reshape(-1, C)
+    if x2.numel() >= 2 ** 31 * C:
+        raise RuntimeError(f'{what}: at most 2^31 - 1 rows')
+    if (C > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < C):
+        x2 = x2.contiguous()
+    return x2, (x2.stride(0) if x2.shape[0] > 1 else C)
+
+
+class LayerNorm(torch.autograd.Function):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [..., C] (fp32 or bf16, evenly
+    spaced rows are read where they lie); weight and bias fp32 [C] or None, statistics and their gradients fp32.  y is
+    contiguous, of x's type.  One launch forward, two backward (layernorm.hip), sums in a fixed order."""
+
+    @staticmethod
+    @_amp_keep
+    def forward(ctx, x, weight, bias, eps):
+        lib = L.load()
+        _check_device(x, 'layer norm input')
+        C = x.shape[-1] if x.dim() else 0
+        if C == 0:
+            raise RuntimeError(f'layer norm: the last dimension must hold values, got {tuple(x.shape)}')
+        for p, what in ((weight, 'weight'), (bias, 'bias')):
+            if p is not None:
+                _check_device(p, f'layer norm {what}')
+                if p.dtype != torch.float32 or p.shape != (C,):
+                    raise RuntimeError(f'layer norm {what}: fp32 [{C}], got {p.dtype} {tuple(p.shape)}')
+        code = _dt(x)
+        x2, ldx = _rows(x, 'layer norm')
+        d = L.NormDesc(x2.shape[0], C, ldx, float(eps), code)
+        weight = weight.contiguous() if weight is not None else None
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = rstd = None
+        if any(ctx.needs_input_grad):
+            mean, rstd = torch.empty(2, x2.shape[0], dtype=torch.float32, device=x.device)
+        L.check(lib.vfd_layer_norm_fwd(ctypes.byref(d), x2.data_ptr(), L.ptr(weight),
+                                       L.ptr(bias.contiguous() if bias is not None else None), y.data_ptr(), L.ptr(mean),
+                                       L.ptr(rstd), L.stream()), 'layer_norm_fwd')
+        if L.PROF_ON:
+            L.ALG_BYTES['layer_norm_fwd'] += 2 * x.numel() * x.element_size()
+        ctx.d = (d.rows, d.cols, d.ldx, d.eps, d.dtype)
+        ctx.save_for_backward(x2, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    @_amp_bwd
+    def backward(ctx, g):
+        lib = L.load()
+        x, weight, mean, rstd = ctx.saved_tensors
+        d = L.NormDesc(*ctx.d)
+        need = ctx.needs_input_grad
+        shape, g = g.shape, g.to(x.dtype).contiguous()
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need[0] else None
+        dw = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need[1] else None
+        db = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need[2] else None
+        nws = lib.vfd_layer_norm_bwd_workspace(ctypes.byref(d)) if need[1] or need[2] else 0
+        ws = _ws(nws, x.device)
+        L.check(lib.vfd_layer_norm_bwd(ctypes.byref(d), g.data_ptr(), x.data_ptr(), L.ptr(weight), mean.data_ptr(),
+                                       rstd.data_ptr(), L.ptr(dx), L.ptr(dw), L.ptr(db), ws.data_ptr(), nws, L.stream()),
+                'layer_norm_bwd')
+        if L.PROF_ON:
+            L.ALG_BYTES['layer_norm_bwd'] += (2 + (dx is not None)) * g.numel() * g.element_size()
+        return dx, dw, db, None
+
+
+# =============================================================================================
+# Linear layer with bias, activation and residual in the product's epilogue
+# =============================================================================================
+class LinearAct(torch.autograd.Function):
+    """y = act(x weight^T + bias) + residual for x [..., K] (evenly spaced rows are read where they lie), weight [N, K],
+    bias [N] or None, residual [..., N] or None, all fp32 or all bf16 (sums in fp32, every output rounded once; bf16
+    keeps the pre-activation and its gradient in bf16 between forward and backward).  act: 'none', 'relu', 'lrelu'
+    (slope 0.1), 'elu', 'gelu' (erf), 'silu'.  One product kernel forward, one for each of d x and d weight backward
+    (linear.hip), sums in a fixed order."""
+
+    @staticmethod
+    @_amp_keep
+    def forward(ctx, x, weight, bias, residual, act):
+        lib = L.load()
+        _check_device(x, 'linear input')
+        if act not in L.LINEAR_ACTS:
+            raise ValueError(f'linear: act is one of {", ".join(L.LINEAR_ACTS)}, got {act!r}')
+        if not torch.is_tensor(weight) or weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or not weight.numel():
+            raise RuntimeError(f'linear: x [..., K] and weight [N, K], K and N at least 1, got {tuple(x.shape)} and '
+                               f'{tuple(getattr(weight, "shape", ()))}')
+        N, K = weight.shape
+        code = _dt(x)
+        for t, what, shape in ((weight, 'weight', (N, K)), (bias, 'bias', (N,)),
+                               (residual, 'residual', (*x.shape[:-1], N))):
+            if t is not None:
+                _check_device(t, f'linear {what}')
+                if t.dtype != x.dtype or t.shape != shape:
+                    raise RuntimeError(f'linear {what}: {x.dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}')
+        x2, ldx = _rows(x, 'linear')
+        d = L.LinearDesc(x2.shape[0], K, N, L.LINEAR_ACTS[act], ldx, code)
+        weight = weight.contiguous()
+        bias = bias.contiguous() if bias is not None else None
+        residual = residual.contiguous() if residual is not None else None
+        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        keep = d.act != 0 and any(ctx.needs_input_grad[:3])
+        z = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device) if keep else None
+        nws = lib.vfd_linear_workspace(ctypes.byref(d), L.LINEAR_FWD)
+        ws = _ws(nws, x.device) if nws else None
+        L.check(lib.vfd_linear_fwd(ctypes.byref(d), x2.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(residual),
+                                   y.data_ptr(), L.ptr(z), L.ptr(ws), nws, L.stream()), 'linear_fwd')
+        if L.PROF_ON:
+            L.ALG_BYTES['linear_fwd'] += x.element_size() * (x.numel() + weight.numel() + y.numel()
+                                                             * (1 + (z is not None) + (residual is not None)))
+        ctx.d = (d.rows, d.k, d.n, d.act, d.ldx, d.dtype)
+        ctx.save_for_backward(x2, weight, z)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    @_amp_bwd
+    def backward(ctx, g):
+        lib = L.load()
+        x, weight, z = ctx.saved_tensors
+        d = L.LinearDesc(*ctx.d)
+        need = ctx.needs_input_grad
+        lead = g.shape[:-1]
+        g = g.to(x.dtype).contiguous()
+        new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)  # noqa: E731
+
+        def call(fn, what, *args):
+            nws = lib.vfd_linear_workspace(ctypes.byref(d), what)
+            ws = _ws(nws, x.device) if nws else None
+            L.check(fn(ctypes.byref(d), *args, L.ptr(ws), nws, L.stream()), fn.__name__)
+        db = new(d.n) if need[2] else None
+        gz = g
+        if any(need[:3]) and (d.act != 0 or need[2]):
+            gz = new(d.rows, d.n) if d.act else g
+            call(lib.vfd_linear_act_bwd, L.LINEAR_ACT_BWD, g.data_ptr(), L.ptr(z), gz.data_ptr(), L.ptr(db))
+        dx = dw = None
+        if need[0]:
+            dx = new(*lead, d.k)
+            call(lib.vfd_linear_dgrad, L.LINEAR_DGRAD, gz.data_ptr(), weight.data_ptr(), dx.data_ptr())
+        if need[1]:
+            dw = new(d.n, d.k)
+            call(lib.vfd_linear_wgrad, L.LINEAR_WGRAD, gz.data_ptr(), x.data_ptr(), dw.data_ptr())
+        if L.PROF_ON:
+            L.ALG_BYTES['linear_bwd'] += x.element_size() * (g.numel() * (1 + 2 * (d.act != 0)) + (need[0] + need[1])
+                                                             * (g.numel() + x.numel() + weight.numel()))
+        return dx, dw, db, (g if need[3] else None), None
+
+
+# =============================================================================================
+# Global gradient norm and clipping (between the backward pass and the optimizer's step)
+# =============================================================================================
+_CLIP_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _dense(t):
+    """Every element of t's memory range exactly once, in some order of the dimensions."""
+    if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
+        return True
+    expect = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _clip_list(tensors, what):
+    """Checked list of gradient tensors: strided fp32 / bf16 tensors on the current HIP device."""
+    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
+    dev = None
+    for t in tensors:
+        if not torch.is_tensor(t) or not t.is_cuda or t.get_device() != dev:
+            _check_device(t, what)
+            dev = t.get_device()
+        if t.dtype not in _CLIP_DTYPES or t.layout is not torch.strided:
+            raise RuntimeError(f'{what}: strided fp32 or bf16 tensors, got {t.dtype} ({t.layout})')
+    return tensors
+
+
+def _clip_call(fn, tensors, norm_type, extra=(), outs=None):
+    """One C call over a list: (pointers, lengths, types) as host arrays, the norm and the partials' workspace."""
+    lib = L.load()
+    if norm_type not in (2, math.inf):
+        raise ValueError(f'{fn}: norm_type 2 or inf, got {norm_type!r}')
+    n = len(tensors)
+    device = tensors[0].device if n else torch.device('cuda', torch.cuda.current_device())
+    ptrs = array.array('Q', [t.data_ptr() for t in tensors])
+    numel = array.array('q', [t.numel() for t in tensors])
+    codes = bytes([_CLIP_DTYPES[t.dtype] for t in tensors])
+    at = lambda a: a.buffer_info()[0]  # noqa: E731
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nws = lib.vfd_grad_norm_workspace(n, at(numel))
+    ws = _ws(nws, device)
+    args = [n, at(ptrs), at(numel), codes, int(norm_type == math.inf), *extra]
+    if fn == 'clip_grads':
+        if outs is None:
+            args += [None, None]
+        else:
+            optrs = array.array('Q', [t.data_ptr() for t in outs])
+            args += [at(optrs), bytes([_CLIP_DTYPES[t.dtype] for t in outs])]
+    L.check(getattr(lib, 'vfd_' + fn)(*args, norm.data_ptr(), ws.data_ptr(), nws, L.stream()), fn)
+    if L.PROF_ON:                            # compulsory: the gradients once, the clipped ones once
+        L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in tensors)
+        L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in (outs or ()))
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type=2.0):
+    """Global norm of a list of gradient tensors (fp32 / bf16, mixed at will) as a 0-d fp32 tensor on the device:
+    sqrt of the sum of all squares, or the largest magnitude for norm_type inf.  Summed in fp64 in a fixed order;
+    nothing waits on the host.  An empty list gives 0."""
+    tensors = _clip_list(grads, 'grad_norm')
+    return _clip_call('grad_norm', [t if _dense(t) else t.contiguous() for t in tensors], norm_type)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """Scale a list of gradient tensors by min(1, max_norm / (norm + 1e-6)), norm their global norm (`grad_norm`),
+    which is returned.  In place (gradients that need no clipping are only read), or, with `out`, into those tensors
+    (same shapes, fp32 or bf16 each: bf16 gradients into an optimizer's fp32 buffers), the gradients left as they
+    are.  max_norm is a host number (a captured graph keeps it).  A NaN norm makes every gradient NaN, an infinite
+    one makes finite gradients 0, as torch.nn.utils.clip_grad_norm_.  Tensors that are written must not share memory
+    with each other or, with `out`, with a gradient."""
+    tensors = _clip_list(grads, 'clip_grads')
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f'clip_grads: max_norm must be a number >= 0, got {max_norm}')
+    if out is None:
+        if not all([_dense(t) for t in tensors]):
+            raise ValueError('clip_grads: a gradient that is not stored densely is clipped into `out`, not in place')
+        norm = _clip_call('clip_grads', tensors, norm_type, (max_norm,))
+    else:
+        outs = _clip_list(out, 'clip_grads out')
+        if len(outs) != len(tensors):
+            raise ValueError(f'clip_grads: {len(tensors)} gradients, {len(outs)} outputs')
+        work = []
+        for t, o in zip(tensors, outs):
+            if t.shape != o.shape:
+                raise ValueError(f'clip_grads: gradient {tuple(t.shape)} into output {tuple(o.shape)}')
+            if not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _dense(t)):
+                if not o.is_contiguous():
+                    raise ValueError('clip_grads: an output is contiguous or laid out as its gradient')
+                t = t.contiguous()
+            work.append(t)
+        norm = _clip_call('clip_grads', work, norm_type, (max_norm,), outs)
+        tensors = outs
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """torch.nn.utils.clip_grad_norm_ on the HIP kernels: clip the .grad of every parameter that has one, in place,
+    to the global norm max_norm; the norm before clipping is returned (0-d, on the device).  A parameter listed twice
+    counts once."""
+    parameters = [parameters] if torch.is_tensor(parameters) else parameters
+    seen = {}
+    for p in parameters:
+        if p.grad is not None:
+            seen[id(p)] = p.grad
+    return clip_grads(list(seen.values()), max_norm, norm_type)

@@ -147,6 +147,54 @@ def max_pool_stem(pool, x):
     return pool(x)
 
 
+def layer_norm(ln, x):
+    """nn.LayerNorm `ln` over the last dimension of x [..., C]: the HIP kernel pair (layernorm.hip) for fp32 or bf16
+    activations on the GPU (parameters and statistics fp32, the output in x's type), the module otherwise (CPU, other
+    types, several normalised dimensions)."""
+    if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and len(ln.normalized_shape) == 1 and x.dim() >= 1
+            and x.shape[-1] == ln.normalized_shape[0]):
+        from . import kernels as KN
+        w, b = (None if p is None else p.float() for p in (ln.weight, ln.bias))
+        return KN.LayerNorm.apply(x, w, b, ln.eps)
+    return ln(x)
+
+
+def channel_norm(ln, x):
+    """`layer_norm` over the channels of each pixel of a map [N, C, H, W]; the output is channels-last.  A
+    channels-last map is read where it lies, another one is copied into that layout first."""
+    return layer_norm(ln, x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+
+
+_ACTS = {'none': lambda z: z, 'relu': F.relu, 'lrelu': lambda z: F.leaky_relu(z, 0.1), 'elu': F.elu, 'gelu': F.gelu,
+         'silu': F.silu}
+
+
+def linear_act(lin, x, act='none', residual=None):
+    """act(lin(x)) + residual for `lin` an nn.Linear (x [..., K]) or a 1x1 nn.Conv2d (x a map [N, K, H, W]): the product
+    with bias, activation and residual in its epilogue (linear.hip) for fp32 or bf16 on the GPU, under autocast in its
+    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types).  act: 'none',
+    'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The convolution's output is channels-last; a channels-last map
+    is read where it lies, another one is copied into that layout first."""
+    if act not in _ACTS:
+        raise ValueError(f'linear_act: act is one of {", ".join(_ACTS)}, got {act!r}')
+    conv = isinstance(lin, nn.Conv2d)
+    if conv and not (tuple(lin.kernel_size) == (1, 1) and tuple(lin.stride) == (1, 1) and lin.groups == 1
+                     and lin.padding in (0, (0, 0), 'valid', 'same') and x.dim() == 4):
+        raise ValueError('linear_act: a convolution is 1x1, of stride 1, without padding or groups, on a map [N, K, H, W]')
+    dt = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else x.dtype
+    if not (x.is_cuda and dt in (torch.float32, torch.bfloat16)):
+        y = _ACTS[act](lin(x))
+        return y if residual is None else y + residual
+    from . import kernels as KN
+    w, b = lin.weight, lin.bias
+    if torch.is_autocast_enabled('cuda'):
+        x, w, b, residual = (None if t is None else t.to(dt) for t in (x, w, b, residual))
+    if not conv:
+        return KN.LinearAct.apply(x, w, b, residual, act)
+    r = residual.permute(0, 2, 3, 1) if residual is not None else None
+    return KN.LinearAct.apply(x.permute(0, 2, 3, 1), w.flatten(1), b, r, act).permute(0, 3, 1, 2)
+
+
 class BasicBlock(nn.Module):
     expansion = 1
 

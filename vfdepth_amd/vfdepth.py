@@ -27,6 +27,7 @@ from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.data import DataLoader
 
 from . import fusion
+from . import kernels as KN
 from .config import flatten
 from .geometry import Pose, ViewRendering, inverse4x4
 from .losses import DepthSynLoss, MultiCamLoss, SingleCamLoss
@@ -128,6 +129,10 @@ class VFDepthAlgo:
             os.environ.setdefault('MIOPEN_DEBUG_CONVOLUTION_DETERMINISTIC', '1')
         if getattr(self, 'net_precision', 'fp32') not in ('fp32', 'bf16'):
             raise ValueError(f'net_precision must be fp32 or bf16, got {self.net_precision!r}')
+        self.max_grad_norm = float(getattr(self, 'max_grad_norm', 0.0) or 0.0)
+        if not self.max_grad_norm >= 0:
+            raise ValueError(f'max_grad_norm must be a number >= 0 (0: no clipping), got {self.max_grad_norm!r}')
+        self.grad_norm = None
         self.prepare_dataset(cfg, rank)
         self.models = self.prepare_model(cfg, rank)
         self.losses = self.init_losses(cfg, rank)
@@ -412,8 +417,21 @@ class VFDepthAlgo:
         return losses
 
     # ------------------------------------------------------------------ HIP graph
+    def clip_gradients(self):
+        """Clip the gradients of every optimized parameter to the global norm `training.max_grad_norm` (0, the
+        default: nothing is done), between backward and the optimizer's step.  The norm before clipping stays in
+        `self.grad_norm` (0-d tensor on the device; a captured step refreshes its own at every replay).  Under DDP the
+        gradients are averaged by then, so every rank finds the same norm."""
+        if not self.max_grad_norm:
+            return
+        params = [p for group in self.optimizer.param_groups for p in group['params']]
+        if self.device.type == 'cuda':
+            self.grad_norm = KN.clip_grad_norm_(params, self.max_grad_norm)
+        else:
+            self.grad_norm = torch.nn.utils.clip_grad_norm_(params, self.max_grad_norm)
+
     def train_step(self, inputs):
-        """zero_grad -> process_batch -> backward -> optimizer step (vfdepth_trainer.py:63-66).
+        """zero_grad -> process_batch -> backward (-> clip_gradients) -> optimizer step (vfdepth_trainer.py:63-66).
         Returns the losses DETACHED: a caller that keeps them (a logger, the bench) must not keep the
         step's autograd graph alive — its AccumulateGrad nodes, and the streams they were created
         on, would otherwise carry into later steps (and into a graph capture)."""
@@ -421,6 +439,7 @@ class VFDepthAlgo:
         _, losses = self.process_batch(inputs, self.rank)
         losses['total_loss'].backward()
         self._join_branch()
+        self.clip_gradients()
         self.optimizer.step()
         return {k: (v.detach() if torch.is_tensor(v) else v) for k, v in losses.items()}
 
@@ -505,6 +524,7 @@ class VFDepthAlgo:
                     static_losses['total_loss'].backward()
                     _trace('captured backward', sync=False)
                     self._join_branch()
+                    self.clip_gradients()
                     self.optimizer.step()
                     _trace('captured optimizer step', sync=False)
                 except BaseException:
@@ -533,6 +553,7 @@ class VFDepthAlgo:
 
         step.graph = graph
         step.outputs = static_outputs      # refreshed by every replay
+        step.grad_norm = self.grad_norm    # likewise (None without max_grad_norm)
         return step
 
     def compute_depth_metrics(self, inputs, outputs, vis_scale=False):
