@@ -131,6 +131,33 @@ struct LinTile {
       *reinterpret_cast<typename X::avec*>(lds + (MC ? at(e / CPR, e % CPR) : at(e >> 3, e & 7))) = v[i];
     }
   }
+  // Whole tiles straight into LDS: a wave's 64 chunks land one after another, so lane l of chunk group e fetches the chunk
+  // whose place that is.  Outer indices beyond the operand fetch its last chunk again (their products are not stored).
+  struct Stream {
+    const T* p[NCH];
+  };
+  static __device__ __forceinline__ void open(const LinOp<T>& op, int o0, int k0, Stream& s) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int e = (int)threadIdx.x + i * NT;
+      const int row = MC ? e / CPR : e >> 3, at = MC ? e % CPR : e & 7;
+      const int c = MC ? (sizeof(T) == 2 ? (at ^ ((row & 3) << 1)) : at) : (at ^ (row & 7));
+      if constexpr (MC)
+        s.p[i] = op.p + (size_t)(k0 + row) * op.ld + min(o0 + c * X::VE, op.O - X::VE);
+      else
+        s.p[i] = op.p + (size_t)min(o0 + row, op.O - 1) * op.ld + k0 + c * X::VE;
+    }
+  }
+  static __device__ __forceinline__ void next(const LinOp<T>& op, Stream& s, char* lds) {
+    typedef const __attribute__((address_space(1))) void gvoid;
+    typedef __attribute__((address_space(3))) void lvoid;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      __builtin_amdgcn_global_load_lds((gvoid*)s.p[i], (lvoid*)(lds + (i * NT + wave * 64) * 16), 16, 0, 0);
+      s.p[i] += MC ? (size_t)X::BK * op.ld : (size_t)X::BK;
+    }
+  }
   // The 32 outer indices from o on, contraction step ks (of 4): lane l holds outer l & 31, 16 bytes of contraction
   static __device__ __forceinline__ typename X::avec frag(const char* lds, int o, int ks) {
     const int lane = threadIdx.x & 63;
@@ -165,7 +192,59 @@ struct LinEpi {
   int act;
 };
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN>
+// Eight consecutive values at any element boundary, `cnt` of them (the rest 0); null: 0
+template <typename T>
+__device__ __forceinline__ void lin_ld8(const T* __restrict__ p, int cnt, float (&f)[8]) {
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (p != nullptr && cnt == 8) {
+    const v8 v = *reinterpret_cast<const v8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (p != nullptr && e < cnt) ? ld1(p + e) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void lin_st8(T* __restrict__ p, int cnt, const float (&f)[8]) {
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (cnt == 8) {
+    v8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (T)f[e];
+    *reinterpret_cast<v8*>(p) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < cnt) st1(p + e, f[e]);
+  }
+}
+
+// The epilogue of eight consecutive outputs at element `at` of y
+template <typename T>
+__device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[8], float (&v)[8]) {
+  float res[8];
+  lin_ld8(ep.res ? ep.res + at : nullptr, cnt, res);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  if (ep.z) lin_st8(ep.z + at, cnt, v);
+  auto each = [&](auto act) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = lin_act<decltype(act)::value>(v[e]);
+  };
+  switch (ep.act) {
+    case LIN_RELU: each(std::integral_constant<int, LIN_RELU>()); break;
+    case LIN_LRELU: each(std::integral_constant<int, LIN_LRELU>()); break;
+    case LIN_ELU: each(std::integral_constant<int, LIN_ELU>()); break;
+    case LIN_GELU: each(std::integral_constant<int, LIN_GELU>()); break;
+    case LIN_SILU: each(std::integral_constant<int, LIN_SILU>()); break;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += res[e];
+  lin_st8(ep.y + at, cnt, v);
+}
+
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, bool ASYNC>
 __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep, int tm, int tn, int splits) {
   constexpr int NT = 64 * WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
   typedef LinT<T> X;
@@ -183,7 +262,8 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
   t -= group * GM * tn;
   const int m0 = (g0 + t % gm) * BM, n0 = (t / gm) * BN;
   const int kt = (x.K + X::BK - 1) / X::BK;
-  const int k_lo = (int)((long long)kt * split / splits), k_hi = (int)((long long)kt * (split + 1) / splits);
+  int k_lo = (int)((long long)kt * split / splits);
+  const int k_hi = (int)((long long)kt * (split + 1) / splits);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = (wave % WM) * FM * 32, wn = (wave / WM) * FN * 32;
 
   lin_f16 acc[FM][FN];
@@ -194,21 +274,7 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  typename X::vec vx[TX::NCH], vw[TW::NCH];
-  if (k_lo < k_hi) {
-    TX::fetch(x, m0, k_lo * X::BK, vx);
-    TW::fetch(w, n0, k_lo * X::BK, vw);
-    TX::put(lds, vx);
-    TW::put(lds + BM * 128, vw);
-  }
-  __syncthreads();
-  for (int k = k_lo; k < k_hi; ++k) {
-    const char* cur = lds + ((k - k_lo) & 1) * STAGE;
-    char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
-    if (k + 1 < k_hi) {
-      TX::fetch(x, m0, (k + 1) * X::BK, vx);
-      TW::fetch(w, n0, (k + 1) * X::BK, vw);
-    }
+  auto work = [&](const char* cur) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       typename X::avec fx[FM], fw[FN];
@@ -221,78 +287,128 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = lin_mma(fw[j], fx[i], acc[i][j]);
     }
-    if (k + 1 < k_hi) {
-      TX::put(nxt, vx);
-      TW::put(nxt + BM * 128, vw);
+  };
+  if constexpr (ASYNC) {
+    // whole tiles in flight into one half of LDS while the other is worked on
+    const int k_end = min(k_hi, x.K / X::BK);
+    typename TX::Stream sx;
+    typename TW::Stream sw;
+    TX::open(x, m0, k_lo * X::BK, sx);
+    TW::open(w, n0, k_lo * X::BK, sw);
+    if (k_lo < k_end) {
+      TX::next(x, sx, lds);
+      TW::next(w, sw, lds + BM * 128);
     }
     __syncthreads();
+    for (int k = k_lo; k < k_end; ++k) {
+      char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
+      if (k + 1 < k_end) {
+        TX::next(x, sx, nxt);
+        TW::next(w, sw, nxt + BM * 128);
+      }
+      work(lds + ((k - k_lo) & 1) * STAGE);
+      __syncthreads();
+    }
+    k_lo = max(k_lo, k_end);                             // a last tile that the contraction ends in: staged with masks
+  }
+  {
+    typename X::vec vx[TX::NCH], vw[TW::NCH];
+    if (k_lo < k_hi) {
+      TX::fetch(x, m0, k_lo * X::BK, vx);
+      TW::fetch(w, n0, k_lo * X::BK, vw);
+      TX::put(lds, vx);
+      TW::put(lds + BM * 128, vw);
+    }
+    __syncthreads();
+    for (int k = k_lo; k < k_hi; ++k) {
+      char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
+      if (k + 1 < k_hi) {
+        TX::fetch(x, m0, (k + 1) * X::BK, vx);
+        TW::fetch(w, n0, (k + 1) * X::BK, vw);
+      }
+      work(lds + ((k - k_lo) & 1) * STAGE);
+      if (k + 1 < k_hi) {
+        TX::put(nxt, vx);
+        TW::put(nxt + BM * 128, vw);
+      }
+      __syncthreads();
+    }
   }
 
-  // D of a block: column (lane & 31) = row of y, 4 consecutive columns of y per group of 4 registers
-  const int M = x.O, N = w.O;
-  auto with_act = [&](auto act) {
+  // D of a block: column (lane & 31) = row of y, 4 consecutive columns of y per group of 4 registers.  Each wave turns 32
+  // rows at a time over in its own part of LDS, so that lanes store (and load residuals) 8 consecutive columns, whole
+  // lines of a row together; the rows' pitch of 4 more floats spreads them over the banks.
+  constexpr int COLS = FN * 32, PITCH = COLS + 4, LPR = COLS / 8;
+  static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE, "the waves' output rows fit where the tiles were");
+  float* turn = reinterpret_cast<float*>(lds) + wave * (32 * PITCH);
+  const int M = x.O, N = w.O, col = n0 + wn + (lane % LPR) * 8, cnt = min(max(N - col, 0), 8);
+  float bias[8];
+  lin_ld8(ep.bias && ep.part == nullptr ? ep.bias + col : nullptr, cnt, bias);
+  auto turn_over = [&](auto i) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int m = m0 + wm + 32 * i + (lane & 31);
-      if (m >= M) continue;
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+      for (int q = 0; q < 4; ++q) {
+        lin_f4 v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + wn + 32 * j + 8 * q + 4 * (lane >> 5);
-          const size_t at = (size_t)m * N + n;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (n + e >= N) continue;
-            float v = acc[i][j][4 * q + e];
-            if constexpr (decltype(act)::value < 0) {
-              ep.part[(size_t)split * M * N + at + e] = v;
-            } else {
-              if (ep.bias) v += ld1(ep.bias + n + e);
-              if (ep.z) st1(ep.z + at + e, v);
-              v = lin_act<decltype(act)::value>(v);
-              if (ep.res) v += ld1(ep.res + at + e);
-              st1(ep.y + at + e, v);
-            }
-          }
-        }
-    }
+        for (int e = 0; e < 4; ++e) v[e] = acc[i()][j][4 * q + e];
+        *reinterpret_cast<lin_f4*>(turn + (lane & 31) * PITCH + 32 * j + 8 * q + 4 * (lane >> 5)) = v;
+      }
   };
-  if (ep.part) {
-    with_act(std::integral_constant<int, -1>());
-    return;
-  }
-  switch (ep.act) {
-    case LIN_RELU: with_act(std::integral_constant<int, LIN_RELU>()); break;
-    case LIN_LRELU: with_act(std::integral_constant<int, LIN_LRELU>()); break;
-    case LIN_ELU: with_act(std::integral_constant<int, LIN_ELU>()); break;
-    case LIN_GELU: with_act(std::integral_constant<int, LIN_GELU>()); break;
-    case LIN_SILU: with_act(std::integral_constant<int, LIN_SILU>()); break;
-    default: with_act(std::integral_constant<int, LIN_NONE>()); break;
+#pragma unroll 1
+  for (int i = 0; i < FM; ++i) {                           // one copy of the epilogue's code
+    if (i == 0) turn_over(std::integral_constant<int, 0>());
+    if constexpr (FM > 1)
+      if (i == 1) turn_over(std::integral_constant<int, 1>());
+    if constexpr (FM > 2) {
+      if (i == 2) turn_over(std::integral_constant<int, 2>());
+      if (i == 3) turn_over(std::integral_constant<int, 3>());
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += 64 / LPR) {
+      const int m = m0 + wm + 32 * i + r;
+      if (m >= M) break;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = turn[r * PITCH + (lane % LPR) * 8 + e];
+      const size_t at = (size_t)m * N + col;
+      if (ep.part)
+        lin_st8(ep.part + (size_t)split * M * N + at, cnt, v);
+      else
+        lin_finish(ep, at, cnt, bias, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // A split contraction's partial products, added in split order, and the epilogue.
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, size_t mn, int N) {
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < mn; i += (size_t)gridDim.x * 1024) {
-    float v[4];
-    const int c = mn - i < 4 ? (int)(mn - i) : 4;
+template <typename T>
+__global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int M, int N) {
+  const int rows8 = (N + 7) / 8;                           // eight columns a thread
+  const size_t mn = (size_t)M * N, all = (size_t)M * rows8;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const size_t m = i / rows8;
+    const int col = (int)(i - m * rows8) * 8, cnt = min(N - col, 8);
+    const float* p = ep.part + m * N + col;
+    float v[8], a[8], b[8];
+    lin_ld8(p, cnt, v);
+    int k = 1;
+    for (; k + 1 < splits; k += 2) {
+      lin_ld8(p + k * mn, cnt, a);
+      lin_ld8(p + (k + 1) * mn, cnt, b);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = 0.f;
-    for (int s = 0; s < splits; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < c) v[e] += ep.part[(size_t)s * mn + i + e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e >= c) continue;
-      if (ep.bias) v[e] += ld1(ep.bias + (i + e) % N);
-      if (ep.z) st1(ep.z + i + e, v[e]);
-      v[e] = lin_act<ACT>(v[e]);
-      if (ep.res) v[e] += ld1(ep.res + i + e);
-      st1(ep.y + i + e, v[e]);
+      for (int e = 0; e < 8; ++e) v[e] = (v[e] + a[e]) + b[e];
     }
+    if (k < splits) {
+      lin_ld8(p + k * mn, cnt, a);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += a[e];
+    }
+    lin_ld8(ep.bias ? ep.bias + col : nullptr, cnt, b);
+    lin_finish(ep, m * N + col, cnt, b, v);
   }
 }
 
@@ -373,34 +489,50 @@ static LinPlan lin_plan(int M, int N, int K, int resident) {
   return p;
 }
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN>
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, bool ASYNC>
 static int lin_launch(const LinOp<T>& x, const LinOp<T>& w, LinEpi<T> ep, const LinPlan& p, float* part, hipStream_t s) {
-  auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN>;
+  auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN, ASYNC>;
   constexpr int bytes = 2 * (BM + BN) * 128;
   lds_attr((const void*)fn, bytes);
   ep.part = p.splits > 1 ? part : nullptr;
   fn<<<(unsigned)(p.tm * p.tn * p.splits), 64 * WM * WN, bytes, s>>>(x, w, ep, p.tm, p.tn, p.splits);
   if (p.splits > 1) {
-    const size_t mn = (size_t)x.O * w.O;
-    const size_t blocks = (mn + 1023) / 1024;
-    lin_with_act(ep.act, [&](auto act) {
-      lin_join_k<T, act()><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, mn, w.O);
-      return 0;
-    });
+    const size_t blocks = ((size_t)x.O * ((w.O + 7) / 8) + 255) / 256;
+    lin_join_k<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, x.O, w.O);
   }
   return fail_launch("linear");
 }
 
-constexpr int LIN_BM = 128, LIN_BN = 128, LIN_RES = 2;
+// Chunks of 16 bytes at 16-byte boundaries everywhere: what the loads that go straight into LDS take.
+template <typename T, bool MC>
+static bool lin_aligned(const LinOp<T>& op) {
+  constexpr int VE = LinT<T>::VE;
+  return ((uintptr_t)op.p & 15) == 0 && op.ld % VE == 0 && (!MC || op.O % VE == 0);
+}
+
+// bf16 products with enough 256 x 256 tiles to fill the chip take them (half the LDS reads a product of 128 x 128 tiles)
+template <typename T>
+static bool lin_big(int M, int N) {
+  return sizeof(T) == 2 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= LIN_CUS;
+}
+
+template <typename T, bool XMC, bool WMC, bool ASYNC>
+static int lin_sized(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, float* part, hipStream_t s) {
+  if constexpr (sizeof(T) == 2 && ASYNC)
+    if (lin_big<T>(x.O, w.O))
+      return lin_launch<T, XMC, WMC, 256, 256, 2, 4, ASYNC>(x, w, ep, lin_plan<T, 256, 256>(x.O, w.O, x.K, 1), part, s);
+  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, ASYNC>(x, w, ep, lin_plan<T, 128, 128>(x.O, w.O, x.K, 2), part, s);
+}
 
 template <typename T, bool XMC, bool WMC>
 static int lin_product(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, float* part, hipStream_t s) {
-  return lin_launch<T, XMC, WMC, LIN_BM, LIN_BN, 2, 2>(x, w, ep, lin_plan<T, LIN_BM, LIN_BN>(x.O, w.O, x.K, LIN_RES), part, s);
+  if (lin_aligned<T, XMC>(x) && lin_aligned<T, WMC>(w)) return lin_sized<T, XMC, WMC, true>(x, w, ep, part, s);
+  return lin_sized<T, XMC, WMC, false>(x, w, ep, part, s);
 }
 
 template <typename T>
 static size_t lin_part_bytes(int M, int N, int K) {
-  const LinPlan p = lin_plan<T, LIN_BM, LIN_BN>(M, N, K, LIN_RES);
+  const LinPlan p = lin_plan<T, 128, 128>(M, N, K, 2);
   return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
 }
 
