@@ -222,7 +222,9 @@ def ptr(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    """hipStream_t of the current device's current stream (without building a torch.cuda.Stream object: the small ops'
+    calls are bound by the host)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 KERNEL_IDS = {

@@ -21,13 +21,35 @@ typedef short lin_s4 __attribute__((ext_vector_type(4)));
 enum LinAct { LIN_NONE = 0, LIN_RELU, LIN_LRELU, LIN_ELU, LIN_GELU, LIN_SILU, LIN_ACTS };
 constexpr float LIN_SLOPE = 0.1f;            // the framework's LeakyReLU
 
+// The activations run once per output, behind the matrix cores: a few instructions each.
+__device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), by Abramowitz & Stegun 7.1.26 (Hastings): erfc(x) =
+// t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), within 1.5e-7 for x >= 0.
+__device__ __forceinline__ float lin_phi(float z, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+  e = lin_exp(-0.5f * z * z);
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float q = 0.5f * p * e;
+  return z > 0.f ? 1.f - q : q;
+}
+
+// exp(z) - 1 for z <= 0: its series where the subtraction would cancel
+__device__ __forceinline__ float lin_expm1(float z) {
+  const float s = z * fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f), 1.f);
+  return z > -0.25f ? s : lin_exp(z) - 1.f;
+}
+
 template <int ACT>
 __device__ __forceinline__ float lin_act(float z) {
   if constexpr (ACT == LIN_RELU) return z <= 0.f ? 0.f : z;               // NaN passes
   if constexpr (ACT == LIN_LRELU) return z > 0.f ? z : LIN_SLOPE * z;
-  if constexpr (ACT == LIN_ELU) return z > 0.f ? z : expm1f(z);
-  if constexpr (ACT == LIN_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if constexpr (ACT == LIN_SILU) return z / (1.f + expf(-z));
+  if constexpr (ACT == LIN_ELU) return z > 0.f ? z : lin_expm1(z);
+  if constexpr (ACT == LIN_GELU) {
+    float e;
+    return z * lin_phi(z, e);
+  }
+  if constexpr (ACT == LIN_SILU) return z * __builtin_amdgcn_rcpf(1.f + lin_exp(-z));
   return z;
 }
 
@@ -35,11 +57,14 @@ template <int ACT>
 __device__ __forceinline__ float lin_slope(float z) {
   if constexpr (ACT == LIN_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == LIN_LRELU) return z > 0.f ? 1.f : LIN_SLOPE;
-  if constexpr (ACT == LIN_ELU) return z > 0.f ? 1.f : expf(z);
-  if constexpr (ACT == LIN_GELU)
-    return fmaf(z, expf(-0.5f * z * z) * 0.39894228040143268f, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if constexpr (ACT == LIN_ELU) return z > 0.f ? 1.f : lin_exp(z);
+  if constexpr (ACT == LIN_GELU) {
+    float e;
+    const float phi = lin_phi(z, e);
+    return fmaf(z, e * 0.39894228040143268f, phi);
+  }
   if constexpr (ACT == LIN_SILU) {
-    const float s = 1.f / (1.f + expf(-z));
+    const float s = __builtin_amdgcn_rcpf(1.f + lin_exp(-z));
     return s * fmaf(z, 1.f - s, 1.f);
   }
   return 1.f;
@@ -61,7 +86,6 @@ static int lin_with_act(int act, F f) {
 template <typename T>
 struct LinT {
   static constexpr int VE = 16 / (int)sizeof(T);        // values of a 16-byte chunk
-  static constexpr int BK = 128 / (int)sizeof(T);       // contraction values of a staged tile
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
   typedef T avec __attribute__((ext_vector_type(16 / sizeof(T))));
 };
@@ -84,28 +108,35 @@ struct LinOp {
   int O, K;
 };
 
-// A tile of BO outer by BK contraction values in LDS, BO * 128 bytes.
-//   MC = false: rows of 128 bytes, one per outer index; 16-byte chunk c of row o lies at chunk c ^ (o & 7), so that the
-//     8 rows a group of lanes reads at one chunk fall on 8 different bank groups.
-//   MC = true: rows of BO values, one per contraction index, 32-byte pairs of chunks exchanged by (k & 3) (bf16: the
-//     transposing read takes 4 rows at once; fp32 lanes read consecutive values).
-template <typename T, bool MC, int BO, int NT>
+// A tile of BO outer indices by RB bytes of contraction in LDS, filled by NT threads.
+//   MC = false: rows of RB bytes, one per outer index.  A fragment's read takes one 16-byte chunk of 32 rows; the 16 lanes
+//     that share a cycle (of 256 bytes) meet 16 different chunk places because a row's chunk numbers are exchanged by its
+//     place among the rows that start at the same bank.
+//   MC = true: rows of BO values, one per contraction index.  bf16: the transposing read takes 64 bytes of 4 rows in a
+//     cycle, spread over 256 bytes by exchanging 64-byte groups by (row & 3); fp32: lanes read consecutive values.
+template <typename T, bool MC, int BO, int NT, int RB>
 struct LinTile {
   typedef LinT<T> X;
-  static constexpr int NCH = BO * 8 / NT;               // chunks a thread stages
-  static constexpr int CPR = BO / X::VE;                // chunks of a contraction row
-  static_assert(BO * 8 % NT == 0, "whole chunks a thread");
+  static constexpr int BK = RB / (int)sizeof(T);        // contraction values of the tile
+  static constexpr int BYTES = BO * RB, CK = RB / 16;   // its bytes, chunks of an outer index
+  static constexpr int NCH = BO * CK / NT;              // chunks a thread stages
+  static constexpr int CPR = MC ? BO / X::VE : CK;      // chunks of a row in LDS
+  static constexpr int READS = !MC ? 1 : sizeof(T) == 2 ? 2 : 4;   // LDS instructions of a fragment
+  static_assert(BO * CK % NT == 0, "whole chunks a thread");
 
+  static __device__ __forceinline__ int turn(int row) {            // what a row's chunk numbers are exchanged by
+    if constexpr (!MC) return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+    return sizeof(T) == 2 ? (row & 3) << 2 : 0;
+  }
   static __device__ __forceinline__ int at(int row, int c) {       // byte offset of a chunk
-    if constexpr (!MC) return row * 128 + ((c ^ (row & 7)) << 4);
-    return row * (BO * (int)sizeof(T)) + ((sizeof(T) == 2 ? (c ^ ((row & 3) << 1)) : c) << 4);
+    return row * (CPR * 16) + ((c ^ turn(row)) << 4);
   }
   static __device__ __forceinline__ void fetch(const LinOp<T>& op, int o0, int k0, typename X::vec (&v)[NCH]) {
-    const bool whole = o0 + BO <= op.O && k0 + X::BK <= op.K;
+    const bool whole = o0 + BO <= op.O && k0 + BK <= op.K;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int e = (int)threadIdx.x + i * NT;
-      const int row = MC ? e / CPR : e >> 3, c = MC ? e % CPR : e & 7;
+      const int row = e / CPR, c = e % CPR;
       const int o = o0 + (MC ? c * X::VE : row), k = k0 + (MC ? row : c * X::VE);
       const T* p = op.p + (MC ? (size_t)k * op.ld + o : (size_t)o * op.ld + k);
       if (whole) {
@@ -128,37 +159,39 @@ struct LinTile {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int e = (int)threadIdx.x + i * NT;
-      *reinterpret_cast<typename X::avec*>(lds + (MC ? at(e / CPR, e % CPR) : at(e >> 3, e & 7))) = v[i];
+      *reinterpret_cast<typename X::avec*>(lds + at(e / CPR, e % CPR)) = v[i];
     }
   }
-  // Whole tiles straight into LDS: a wave's 64 chunks land one after another, so lane l of chunk group e fetches the chunk
-  // whose place that is.  Outer indices beyond the operand fetch its last chunk again (their products are not stored).
+  // Whole tiles straight into LDS: a wave's 64 chunks land one after another, so each lane fetches the chunk whose place
+  // that is.  Outer indices beyond the operand fetch its last chunk again (their products are not stored).  Through a
+  // buffer descriptor: a lane's offsets stay the same for every tile, and past the last tile an empty one loads nothing.
   struct Stream {
-    const T* p[NCH];
+    const char* p;                                      // of the next tile (uniform)
+    long long step;
+    unsigned off[NCH];
   };
   static __device__ __forceinline__ void open(const LinOp<T>& op, int o0, int k0, Stream& s) {
+    constexpr int ES = (int)sizeof(T);
+    s.p = (const char*)(op.p + (MC ? (size_t)k0 * op.ld + o0 : (size_t)o0 * op.ld + k0));
+    s.step = (long long)BK * ES * (MC ? op.ld : 1);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int e = (int)threadIdx.x + i * NT;
-      const int row = MC ? e / CPR : e >> 3, at = MC ? e % CPR : e & 7;
-      const int c = MC ? (sizeof(T) == 2 ? (at ^ ((row & 3) << 1)) : at) : (at ^ (row & 7));
-      if constexpr (MC)
-        s.p[i] = op.p + (size_t)(k0 + row) * op.ld + min(o0 + c * X::VE, op.O - X::VE);
-      else
-        s.p[i] = op.p + (size_t)min(o0 + row, op.O - 1) * op.ld + k0 + c * X::VE;
+      const int row = e / CPR, c = ((e % CPR) ^ turn(row)) * X::VE;
+      s.off[i] = MC ? (unsigned)row * (unsigned)op.ld * ES + (unsigned)min(c, op.O - X::VE - o0) * ES
+                    : (unsigned)min(row, op.O - 1 - o0) * (unsigned)op.ld * ES + c * ES;
     }
   }
-  static __device__ __forceinline__ void next(const LinOp<T>& op, Stream& s, char* lds) {
-    typedef const __attribute__((address_space(1))) void gvoid;
+  static __device__ __forceinline__ void next(Stream& s, char* lds, bool live) {
     typedef __attribute__((address_space(3))) void lvoid;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)s.p, 0, live ? 0x7fffffff : 0, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      __builtin_amdgcn_global_load_lds((gvoid*)s.p[i], (lvoid*)(lds + (i * NT + wave * 64) * 16), 16, 0, 0);
-      s.p[i] += MC ? (size_t)X::BK * op.ld : (size_t)X::BK;
-    }
+    for (int i = 0; i < NCH; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lvoid*)(lds + (i * NT + wave * 64) * 16), 16, s.off[i], 0, 0, 0);
+    s.p += s.step;
   }
-  // The 32 outer indices from o on, contraction step ks (of 4): lane l holds outer l & 31, 16 bytes of contraction
+  // The 32 outer indices from o on, contraction step ks (32 bytes each): lane l holds outer l & 31, 16 bytes of contraction
   static __device__ __forceinline__ typename X::avec frag(const char* lds, int o, int ks) {
     const int lane = threadIdx.x & 63;
     typename X::avec r;
@@ -176,11 +209,22 @@ struct LinTile {
     } else {
       const int k = 8 * ks + 4 * (lane >> 5);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(lds + (k + j) * (BO * 4) + (o + (lane & 31)) * 4);
+      for (int j = 0; j < 4; ++j) {
+        const int col = o + (lane & 31);
+        r[j] = *reinterpret_cast<const float*>(lds + at(k + j, col >> 2) + (col & 3) * 4);
+      }
     }
     return r;
   }
 };
+
+// Loads straight into LDS are counted with the loads from memory, and a barrier does not wait for them by itself: every
+// wave waits until at most LEFT of its own are on their way (they arrive in order) and its LDS reads have ended, then all
+// wait for each other.
+template <int LEFT>
+__device__ __forceinline__ void lin_arrived() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
 
 template <typename T>
 struct LinEpi {
@@ -221,37 +265,26 @@ __device__ __forceinline__ void lin_st8(T* __restrict__ p, int cnt, const float 
 }
 
 // The epilogue of eight consecutive outputs at element `at` of y
-template <typename T>
-__device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[8], float (&v)[8]) {
-  float res[8];
-  lin_ld8(ep.res ? ep.res + at : nullptr, cnt, res);
+template <int ACT, typename T>
+__device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[8], const float (&res)[8],
+                                           float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
   if (ep.z) lin_st8(ep.z + at, cnt, v);
-  auto each = [&](auto act) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = lin_act<decltype(act)::value>(v[e]);
-  };
-  switch (ep.act) {
-    case LIN_RELU: each(std::integral_constant<int, LIN_RELU>()); break;
-    case LIN_LRELU: each(std::integral_constant<int, LIN_LRELU>()); break;
-    case LIN_ELU: each(std::integral_constant<int, LIN_ELU>()); break;
-    case LIN_GELU: each(std::integral_constant<int, LIN_GELU>()); break;
-    case LIN_SILU: each(std::integral_constant<int, LIN_SILU>()); break;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += res[e];
+  for (int e = 0; e < 8; ++e) v[e] = lin_act<ACT>(v[e]) + res[e];
   lin_st8(ep.y + at, cnt, v);
 }
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, bool ASYNC>
-__global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep, int tm, int tn, int splits) {
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep, int tm, int tn, int splits) {
   constexpr int NT = 64 * WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
   typedef LinT<T> X;
-  typedef LinTile<T, XMC, BM, NT> TX;
-  typedef LinTile<T, WMC, BN, NT> TW;
+  typedef LinTile<T, XMC, BM, NT, RB> TX;
+  typedef LinTile<T, WMC, BN, NT, RB> TW;
+  constexpr int BK = TX::BK, KS = RB / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int STAGE = (BM + BN) * 128;
+  constexpr int STAGE = (BM + BN) * RB, LOADS = TX::NCH + TW::NCH;
   // tiles of one XCD (every eighth workgroup) are consecutive: column groups of 8 row tiles, splits outermost
   const int total = tm * tn * splits, xcd = blockIdx.x % 8, per = total / 8, rest = total % 8;
   int t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
@@ -261,7 +294,7 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
   const int group = t / (GM * tn), g0 = group * GM, gm = min(GM, tm - g0);
   t -= group * GM * tn;
   const int m0 = (g0 + t % gm) * BM, n0 = (t / gm) * BN;
-  const int kt = (x.K + X::BK - 1) / X::BK;
+  const int kt = (x.K + BK - 1) / BK;
   int k_lo = (int)((long long)kt * split / splits);
   const int k_hi = (int)((long long)kt * (split + 1) / splits);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = (wave % WM) * FM * 32, wn = (wave / WM) * FN * 32;
@@ -274,72 +307,119 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto work = [&](const char* cur) {
+  typename X::avec fx[2][FM], fw[2][FN];
+  auto load = [&](auto f, const char* cur, int ks) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      typename X::avec fx[FM], fw[FN];
+    for (int i = 0; i < FM; ++i) fx[f()][i] = TX::frag(cur, wm + 32 * i, ks);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = TX::frag(cur, wm + 32 * i, ks);
+    for (int j = 0; j < FN; ++j) fw[f()][j] = TW::frag(cur + TX::BYTES, wn + 32 * j, ks);
+  };
+  auto mma = [&](auto f) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = TW::frag(cur + BM * 128, wn + 32 * j, ks);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int j = 0; j < FN; ++j) acc[i][j] = lin_mma(fw[f()][j], fx[f()][i], acc[i][j]);
+  };
+  const std::integral_constant<int, 0> f0;
+  const std::integral_constant<int, 1> f1;
+  // A step's instructions in turn: the reads of the next step's fragments (and the loads of another tile) between the
+  // products of this one.  Left to itself the compiler reads fragments just before it needs them and waits.
+  constexpr int READS = FM * TX::READS + FN * TW::READS, MMAS = FM * FN * (sizeof(T) == 2 ? 1 : 4);
+  auto in_turn = [&](auto loads) {
+    constexpr int PARTS = READS < MMAS ? READS : MMAS;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = lin_mma(fw[j], fx[i], acc[i][j]);
+    for (int u = 0; u < PARTS; ++u) {
+      constexpr int rd = 0x100, mm = 0x008, vm = 0x020;
+      __builtin_amdgcn_sched_group_barrier(rd, READS / PARTS, 0);
+      if constexpr (loads() > 0) __builtin_amdgcn_sched_group_barrier(vm, (loads() + PARTS - 1) / PARTS, 0);
+      __builtin_amdgcn_sched_group_barrier(mm, MMAS / PARTS, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const std::integral_constant<int, 0> no_loads;
+  const std::integral_constant<int, LOADS> tile_loads;
+  // all steps of a tile but the last's products; its first fragments are in f0, its last are left in f1
+  auto steps = [&](const char* cur) {
+#pragma unroll
+    for (int ks = 0; ks + 1 < KS; ks += 2) {
+      load(f1, cur, ks + 1);
+      mma(f0);
+      in_turn(no_loads);
+      if (ks + 2 < KS) {
+        load(f0, cur, ks + 2);
+        mma(f1);
+        in_turn(no_loads);
+      }
     }
   };
   if constexpr (ASYNC) {
-    // whole tiles in flight into one half of LDS while the other is worked on
-    const int k_end = min(k_hi, x.K / X::BK);
-    typename TX::Stream sx;
-    typename TW::Stream sw;
-    TX::open(x, m0, k_lo * X::BK, sx);
-    TW::open(w, n0, k_lo * X::BK, sw);
+    // SLOTS tiles in LDS: one is worked on, the others are on their way.  The fragments of a step are read during the
+    // products of the step before; a tile's last products run behind the barrier that frees its slot, while the next
+    // tile's first fragments are read and another tile starts on its way.
+    const int k_end = min(k_hi, x.K / BK);
     if (k_lo < k_end) {
-      TX::next(x, sx, lds);
-      TW::next(w, sw, lds + BM * 128);
-    }
-    __syncthreads();
-    for (int k = k_lo; k < k_end; ++k) {
-      char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
-      if (k + 1 < k_end) {
-        TX::next(x, sx, nxt);
-        TW::next(w, sw, nxt + BM * 128);
+      typename TX::Stream sx;
+      typename TW::Stream sw;
+      TX::open(x, m0, k_lo * BK, sx);
+      TW::open(w, n0, k_lo * BK, sw);
+      auto stage = [&](char* at, bool live) {
+        TX::next(sx, at, live);
+        TW::next(sw, at + TX::BYTES, live);
+      };
+#pragma unroll
+      for (int u = 0; u < SLOTS; ++u) stage(lds + u * STAGE, k_lo + u < k_end);
+      lin_arrived<LOADS * (SLOTS - 1)>();
+      load(f0, lds, 0);
+      int slot = 0;
+#pragma unroll 1
+      for (int k = k_lo; k < k_end; ++k) {
+        char* cur = lds + slot * STAGE;
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        steps(cur);
+        lin_arrived<LOADS * (SLOTS - 2)>();                // the next tile is there
+        stage(cur, k + SLOTS < k_end);
+        load(f0, lds + slot * STAGE, 0);                   // (behind the last tile: read, not used)
+        mma(f1);
+        in_turn(tile_loads);
       }
-      work(lds + ((k - k_lo) & 1) * STAGE);
-      __syncthreads();
+      lin_arrived<0>();
     }
     k_lo = max(k_lo, k_end);                             // a last tile that the contraction ends in: staged with masks
   }
   {
     typename X::vec vx[TX::NCH], vw[TW::NCH];
     if (k_lo < k_hi) {
-      TX::fetch(x, m0, k_lo * X::BK, vx);
-      TW::fetch(w, n0, k_lo * X::BK, vw);
+      TX::fetch(x, m0, k_lo * BK, vx);
+      TW::fetch(w, n0, k_lo * BK, vw);
       TX::put(lds, vx);
-      TW::put(lds + BM * 128, vw);
+      TW::put(lds + TX::BYTES, vw);
     }
     __syncthreads();
     for (int k = k_lo; k < k_hi; ++k) {
       char* nxt = lds + ((k + 1 - k_lo) & 1) * STAGE;
       if (k + 1 < k_hi) {
-        TX::fetch(x, m0, (k + 1) * X::BK, vx);
-        TW::fetch(w, n0, (k + 1) * X::BK, vw);
+        TX::fetch(x, m0, (k + 1) * BK, vx);
+        TW::fetch(w, n0, (k + 1) * BK, vw);
       }
-      work(lds + ((k - k_lo) & 1) * STAGE);
+      const char* cur = lds + ((k - k_lo) & 1) * STAGE;
+      load(f0, cur, 0);
+      steps(cur);
+      mma(f1);
       if (k + 1 < k_hi) {
         TX::put(nxt, vx);
-        TW::put(nxt + BM * 128, vw);
+        TW::put(nxt + TX::BYTES, vw);
       }
       __syncthreads();
     }
   }
 
   // D of a block: column (lane & 31) = row of y, 4 consecutive columns of y per group of 4 registers.  Each wave turns 32
-  // rows at a time over in its own part of LDS, so that lanes store (and load residuals) 8 consecutive columns, whole
-  // lines of a row together; the rows' pitch of 4 more floats spreads them over the banks.
-  constexpr int COLS = FN * 32, PITCH = COLS + 4, LPR = COLS / 8;
-  static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE, "the waves' output rows fit where the tiles were");
+  // rows at a time over in its own part of LDS, so that its lanes store (and load residuals) 8 consecutive columns each,
+  // whole lines of a row together: stored from registers, 32 bytes of 32 rows at a time, the same outputs took up to
+  // twice as long (92 160 x 1024 bf16, contraction 256: 197 us, 120 this way).  The pitch of 4 more floats spreads the
+  // rows over the banks.
+  constexpr int COLS = FN * 32, PITCH = COLS + 4, LPR = COLS / 8, PASS = 64 / LPR;
+  static_assert(WM * WN * 32 * PITCH * 4 <= SLOTS * STAGE, "the waves' output rows fit where the tiles were");
   float* turn = reinterpret_cast<float*>(lds) + wave * (32 * PITCH);
   const int M = x.O, N = w.O, col = n0 + wn + (lane % LPR) * 8, cnt = min(max(N - col, 0), 8);
   float bias[8];
@@ -366,18 +446,31 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += 64 / LPR) {
-      const int m = m0 + wm + 32 * i + r;
-      if (m >= M) break;
-      float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = turn[r * PITCH + (lane % LPR) * 8 + e];
-      const size_t at = (size_t)m * N + col;
-      if (ep.part)
-        lin_st8(ep.part + (size_t)split * M * N + at, cnt, v);
-      else
-        lin_finish(ep, at, cnt, bias, v);
+    for (int r0 = 0; r0 < 32; r0 += 4 * PASS) {            // four rows a lane in flight
+      float v[4][8], res[4][8];
+      int c[4];
+      size_t at[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = r0 + u * PASS + lane / LPR, m = m0 + wm + 32 * i + r;
+        c[u] = m < M ? cnt : 0;
+        at[u] = (size_t)m * N + col;
+        lin_ld8(ep.res && ep.part == nullptr ? ep.res + at[u] : nullptr, c[u], res[u]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const lin_f4 t = *reinterpret_cast<const lin_f4*>(turn + r * PITCH + (lane % LPR) * 8 + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][4 * h + e] = t[e];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (ep.part)
+          lin_st8(ep.part + (size_t)split * M * N + at[u], c[u], v[u]);
+        else
+          lin_finish<ACT>(ep, at[u], c[u], bias, res[u], v[u]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -385,7 +478,7 @@ __global__ __launch_bounds__(64 * WM * WN) void lin_tile_k(LinOp<T> x, LinOp<T> 
 }
 
 // A split contraction's partial products, added in split order, and the epilogue.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int M, int N) {
   const int rows8 = (N + 7) / 8;                           // eight columns a thread
   const size_t mn = (size_t)M * N, all = (size_t)M * rows8;
@@ -408,7 +501,8 @@ __global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int 
       for (int e = 0; e < 8; ++e) v[e] += a[e];
     }
     lin_ld8(ep.bias ? ep.bias + col : nullptr, cnt, b);
-    lin_finish(ep, m * N + col, cnt, b, v);
+    lin_ld8(ep.res ? ep.res + m * N + col : nullptr, cnt, a);
+    lin_finish<ACT>(ep, m * N + col, cnt, b, a, v);
   }
 }
 
@@ -470,6 +564,7 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
 
 // ---------------------------------------------------------------- host
 constexpr int LIN_CUS = 256;
+constexpr int LIN_RB = 128, LIN_SLOTS = 2;   // rings of four or five tiles of 64 bytes: 3 to 20 % slower (16 384 x 2048 x 8192)
 
 struct LinPlan {
   int tm, tn, splits;
@@ -479,35 +574,52 @@ struct LinPlan {
 // split keeps at least four staged tiles of work).
 template <typename T, int BM, int BN>
 static LinPlan lin_plan(int M, int N, int K, int resident) {
+  constexpr int BK = 128 / (int)sizeof(T);
   LinPlan p;
   p.tm = (M + BM - 1) / BM;
   p.tn = (N + BN - 1) / BN;
-  const long long tiles = (long long)p.tm * p.tn, kt = (K + LinT<T>::BK - 1) / LinT<T>::BK;
+  const long long tiles = (long long)p.tm * p.tn, kt = (K + BK - 1) / BK;
   long long s = (long long)LIN_CUS * resident / tiles;
   if (s > kt / 4) s = kt / 4;
   p.splits = s < 1 ? 1 : (int)s;
   return p;
 }
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, bool ASYNC>
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC>
 static int lin_launch(const LinOp<T>& x, const LinOp<T>& w, LinEpi<T> ep, const LinPlan& p, float* part, hipStream_t s) {
-  auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN, ASYNC>;
-  constexpr int bytes = 2 * (BM + BN) * 128;
-  lds_attr((const void*)fn, bytes);
+  constexpr int bytes = SLOTS * (BM + BN) * RB;
   ep.part = p.splits > 1 ? part : nullptr;
-  fn<<<(unsigned)(p.tm * p.tn * p.splits), 64 * WM * WN, bytes, s>>>(x, w, ep, p.tm, p.tn, p.splits);
+  const unsigned grid = (unsigned)(p.tm * p.tn * p.splits);
+  auto launch = [&](auto act) {
+    auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN, OCC, RB, SLOTS, ASYNC, act()>;
+    lds_attr((const void*)fn, bytes);
+    fn<<<grid, 64 * WM * WN, bytes, s>>>(x, w, ep, p.tm, p.tn, p.splits);
+    return 0;
+  };
+  if constexpr (XMC || WMC) {                              // gradients have no activation of their own
+    launch(std::integral_constant<int, LIN_NONE>());
+  } else {
+    if (p.splits > 1)
+      launch(std::integral_constant<int, LIN_NONE>());
+    else
+      lin_with_act(ep.act, launch);
+  }
   if (p.splits > 1) {
     const size_t blocks = ((size_t)x.O * ((w.O + 7) / 8) + 255) / 256;
-    lin_join_k<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, x.O, w.O);
+    lin_with_act(ep.act, [&](auto act) {
+      lin_join_k<T, act()><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, x.O, w.O);
+      return 0;
+    });
   }
   return fail_launch("linear");
 }
 
-// Chunks of 16 bytes at 16-byte boundaries everywhere: what the loads that go straight into LDS take.
+// Chunks of 16 bytes at 16-byte boundaries everywhere, and a tile's rows within 31 bits of bytes: what the loads that go
+// straight into LDS take.
 template <typename T, bool MC>
 static bool lin_aligned(const LinOp<T>& op) {
   constexpr int VE = LinT<T>::VE;
-  return ((uintptr_t)op.p & 15) == 0 && op.ld % VE == 0 && (!MC || op.O % VE == 0);
+  return ((uintptr_t)op.p & 15) == 0 && op.ld % VE == 0 && (!MC || op.O % VE == 0) && op.ld < (1 << 20);
 }
 
 // bf16 products with enough 256 x 256 tiles to fill the chip take them (half the LDS reads a product of 128 x 128 tiles)
@@ -520,8 +632,8 @@ template <typename T, bool XMC, bool WMC, bool ASYNC>
 static int lin_sized(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, float* part, hipStream_t s) {
   if constexpr (sizeof(T) == 2 && ASYNC)
     if (lin_big<T>(x.O, w.O))
-      return lin_launch<T, XMC, WMC, 256, 256, 2, 4, ASYNC>(x, w, ep, lin_plan<T, 256, 256>(x.O, w.O, x.K, 1), part, s);
-  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, ASYNC>(x, w, ep, lin_plan<T, 128, 128>(x.O, w.O, x.K, 2), part, s);
+      return lin_launch<T, XMC, WMC, 256, 256, 2, 2, 1, LIN_RB, LIN_SLOTS, ASYNC>(x, w, ep, lin_plan<T, 256, 256>(x.O, w.O, x.K, 1), part, s);
+  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, LIN_RB, LIN_SLOTS, ASYNC>(x, w, ep, lin_plan<T, 128, 128>(x.O, w.O, x.K, 2), part, s);
 }
 
 template <typename T, bool XMC, bool WMC>

@@ -7,6 +7,7 @@ missing library or a non-HIP tensor raises.
 import array
 import ctypes
 import math
+import operator
 import os
 import weakref
 
@@ -18,6 +19,8 @@ from . import _lib as L
 
 
 def _check_device(t, what):
+    if torch.is_tensor(t) and t.is_cuda and t.get_device() == torch._C._cuda_getDevice():
+        return
     if not torch.is_tensor(t) or not t.is_cuda:
         raise RuntimeError(f'{what}: the VFDepth hot path runs only on a HIP device (got '
                            f'{"non-tensor" if not torch.is_tensor(t) else t.device})')
@@ -2122,15 +2125,32 @@ class MaxPool3s2(torch.autograd.Function):
 # Layer norm over the last dimension
 # =============================================================================================
 def _rows(x, what):
-    """x [..., C] as (rows [R, C] with a unit last stride, elements from one row to the next): a view where x's
-    leading dimensions are evenly spaced, a copy otherwise."""
+    """x [..., C] as (rows with a unit last stride, their number R, elements from one to the next): x itself or a view
+    where its leading dimensions are evenly spaced, a copy otherwise."""
     C = x.shape[-1]
-    x2 = x.reshape(-1, C)
-    if x2.numel() >= 2 ** 31 * C:
+    if x.numel() >= 2 ** 31 * C:
         raise RuntimeError(f'{what}: at most 2^31 - 1 rows')
+    if x.is_contiguous():
+        return x, x.numel() // C, C
+    x2 = x.reshape(-1, C)
     if (C > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < C):
         x2 = x2.contiguous()
-    return x2, (x2.stride(0) if x2.shape[0] > 1 else C)
+    return x2, x2.shape[0], (x2.stride(0) if x2.shape[0] > 1 else C)
+
+
+def _once(fn):
+    """A backward that cannot itself be differentiated: once_differentiable's check, entered only where a graph of the
+    gradients is asked for (it costs the host as much as a small kernel)."""
+    checked = once_differentiable(fn)
+
+    def backward(ctx, g):
+        return checked(ctx, g) if torch.is_grad_enabled() else fn(ctx, g)
+    return staticmethod(backward)
+
+
+def _as(t, like):
+    """An incoming gradient, dense and of the forward's type."""
+    return t if t.dtype == like.dtype and t.is_contiguous() else t.to(like.dtype).contiguous()
 
 
 class LayerNorm(torch.autograd.Function):
@@ -2139,7 +2159,6 @@ class LayerNorm(torch.autograd.Function):
     contiguous, of x's type.  One launch forward, two backward (layernorm.hip), sums in a fixed order."""
 
     @staticmethod
-    @_amp_keep
     def forward(ctx, x, weight, bias, eps):
         lib = L.load()
         _check_device(x, 'layer norm input')
@@ -2152,41 +2171,43 @@ class LayerNorm(torch.autograd.Function):
                 if p.dtype != torch.float32 or p.shape != (C,):
                     raise RuntimeError(f'layer norm {what}: fp32 [{C}], got {p.dtype} {tuple(p.shape)}')
         code = _dt(x)
-        x2, ldx = _rows(x, 'layer norm')
-        d = L.NormDesc(x2.shape[0], C, ldx, float(eps), code)
+        x2, rows, ldx = _rows(x, 'layer norm')
+        d = L.NormDesc(rows, C, ldx, eps, code)
         weight = weight.contiguous() if weight is not None else None
+        bias = bias.contiguous() if bias is not None else None
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = rstd = None
+        stats = m = r = None
         if any(ctx.needs_input_grad):
-            mean, rstd = torch.empty(2, x2.shape[0], dtype=torch.float32, device=x.device)
-        L.check(lib.vfd_layer_norm_fwd(ctypes.byref(d), x2.data_ptr(), L.ptr(weight),
-                                       L.ptr(bias.contiguous() if bias is not None else None), y.data_ptr(), L.ptr(mean),
-                                       L.ptr(rstd), L.stream()), 'layer_norm_fwd')
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)      # means, then 1 / deviations
+            m = stats.data_ptr()
+            r = m + 4 * rows
+        L.check(lib.vfd_layer_norm_fwd(ctypes.byref(d), x2.data_ptr(), L.ptr(weight), L.ptr(bias), y.data_ptr(), m, r,
+                                       L.stream()), 'layer_norm_fwd')
         if L.PROF_ON:
             L.ALG_BYTES['layer_norm_fwd'] += 2 * x.numel() * x.element_size()
-        ctx.d = (d.rows, d.cols, d.ldx, d.eps, d.dtype)
-        ctx.save_for_backward(x2, weight, mean, rstd)
+        ctx.d = d
+        ctx.save_for_backward(x2, weight, stats)
         return y
 
-    @staticmethod
-    @once_differentiable
-    @_amp_bwd
+    @_once
     def backward(ctx, g):
         lib = L.load()
-        x, weight, mean, rstd = ctx.saved_tensors
-        d = L.NormDesc(*ctx.d)
-        need = ctx.needs_input_grad
-        shape, g = g.shape, g.to(x.dtype).contiguous()
-        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need[0] else None
-        dw = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need[1] else None
-        db = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need[2] else None
-        nws = lib.vfd_layer_norm_bwd_workspace(ctypes.byref(d)) if need[1] or need[2] else 0
-        ws = _ws(nws, x.device)
-        L.check(lib.vfd_layer_norm_bwd(ctypes.byref(d), g.data_ptr(), x.data_ptr(), L.ptr(weight), mean.data_ptr(),
-                                       rstd.data_ptr(), L.ptr(dx), L.ptr(dw), L.ptr(db), ws.data_ptr(), nws, L.stream()),
-                'layer_norm_bwd')
+        x, weight, stats = ctx.saved_tensors
+        d = ctx.d
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        g = _as(g, x)
+        dx = torch.empty_like(g) if need_x else None
+        dw = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need_w else None
+        db = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need_b else None
+        ws, nws = None, 0
+        if need_w or need_b:
+            nws = lib.vfd_layer_norm_bwd_workspace(ctypes.byref(d))
+            ws = _ws(nws, x.device)
+        m = stats.data_ptr()
+        L.check(lib.vfd_layer_norm_bwd(ctypes.byref(d), g.data_ptr(), x.data_ptr(), L.ptr(weight), m, m + 4 * d.rows,
+                                       L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), nws, L.stream()), 'layer_norm_bwd')
         if L.PROF_ON:
-            L.ALG_BYTES['layer_norm_bwd'] += (2 + (dx is not None)) * g.numel() * g.element_size()
+            L.ALG_BYTES['layer_norm_bwd'] += (2 + need_x) * g.numel() * g.element_size()
         return dx, dw, db, None
 
 
@@ -2201,7 +2222,6 @@ class LinearAct(torch.autograd.Function):
     (linear.hip), sums in a fixed order."""
 
     @staticmethod
-    @_amp_keep
     def forward(ctx, x, weight, bias, residual, act):
         lib = L.load()
         _check_device(x, 'linear input')
@@ -2218,14 +2238,14 @@ class LinearAct(torch.autograd.Function):
                 _check_device(t, f'linear {what}')
                 if t.dtype != x.dtype or t.shape != shape:
                     raise RuntimeError(f'linear {what}: {x.dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}')
-        x2, ldx = _rows(x, 'linear')
-        d = L.LinearDesc(x2.shape[0], K, N, L.LINEAR_ACTS[act], ldx, code)
+        x2, rows, ldx = _rows(x, 'linear')
+        d = L.LinearDesc(rows, K, N, L.LINEAR_ACTS[act], ldx, code)
         weight = weight.contiguous()
         bias = bias.contiguous() if bias is not None else None
         residual = residual.contiguous() if residual is not None else None
         y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
         keep = d.act != 0 and any(ctx.needs_input_grad[:3])
-        z = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device) if keep else None
+        z = torch.empty(rows, N, dtype=x.dtype, device=x.device) if keep else None
         nws = lib.vfd_linear_workspace(ctypes.byref(d), L.LINEAR_FWD)
         ws = _ws(nws, x.device) if nws else None
         L.check(lib.vfd_linear_fwd(ctypes.byref(d), x2.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(residual),
@@ -2233,20 +2253,18 @@ class LinearAct(torch.autograd.Function):
         if L.PROF_ON:
             L.ALG_BYTES['linear_fwd'] += x.element_size() * (x.numel() + weight.numel() + y.numel()
                                                              * (1 + (z is not None) + (residual is not None)))
-        ctx.d = (d.rows, d.k, d.n, d.act, d.ldx, d.dtype)
+        ctx.d = d
         ctx.save_for_backward(x2, weight, z)
         return y
 
-    @staticmethod
-    @once_differentiable
-    @_amp_bwd
+    @_once
     def backward(ctx, g):
         lib = L.load()
         x, weight, z = ctx.saved_tensors
-        d = L.LinearDesc(*ctx.d)
+        d = ctx.d
         need = ctx.needs_input_grad
         lead = g.shape[:-1]
-        g = g.to(x.dtype).contiguous()
+        g = _as(g, x)
         new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)  # noqa: E731
 
         def call(fn, what, *args):
@@ -2289,17 +2307,33 @@ def _dense(t):
     return True
 
 
+_dtype_of, _layout_of, _shape_of = (operator.attrgetter(a) for a in ('dtype', 'layout', 'shape'))
+
+
 def _clip_list(tensors, what):
     """Checked list of gradient tensors: strided fp32 / bf16 tensors on the current HIP device."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    dev = None
+    # whole-list passes (a model has hundreds of gradients, and the kernels take tens of microseconds), tensor by tensor
+    # only to name the one that does not fit
+    if all(map(torch.is_tensor, tensors)) and not set(map(torch.Tensor.get_device, tensors)) - {_current_device(tensors)} \
+            and set(map(_dtype_of, tensors)) <= _CLIP_DTYPES.keys() and set(map(_layout_of, tensors)) <= {torch.strided}:
+        return tensors
     for t in tensors:
-        if not torch.is_tensor(t) or not t.is_cuda or t.get_device() != dev:
-            _check_device(t, what)
-            dev = t.get_device()
+        _check_device(t, what)
         if t.dtype not in _CLIP_DTYPES or t.layout is not torch.strided:
             raise RuntimeError(f'{what}: strided fp32 or bf16 tensors, got {t.dtype} ({t.layout})')
     return tensors
+
+
+def _current_device(tensors):
+    return torch._C._cuda_getDevice() if any(t.is_cuda for t in tensors[:1]) else None
+
+
+def _clip_codes(tensors):
+    kinds = set(map(_dtype_of, tensors))
+    if len(kinds) == 1:
+        return bytes([_CLIP_DTYPES[kinds.pop()]]) * len(tensors)
+    return bytes([_CLIP_DTYPES[t.dtype] for t in tensors])
 
 
 def _clip_call(fn, tensors, norm_type, extra=(), outs=None):
@@ -2309,20 +2343,19 @@ def _clip_call(fn, tensors, norm_type, extra=(), outs=None):
         raise ValueError(f'{fn}: norm_type 2 or inf, got {norm_type!r}')
     n = len(tensors)
     device = tensors[0].device if n else torch.device('cuda', torch.cuda.current_device())
-    ptrs = array.array('Q', [t.data_ptr() for t in tensors])
-    numel = array.array('q', [t.numel() for t in tensors])
-    codes = bytes([_CLIP_DTYPES[t.dtype] for t in tensors])
+    ptrs = array.array('Q', map(torch.Tensor.data_ptr, tensors))
+    numel = array.array('q', map(torch.Tensor.numel, tensors))
     at = lambda a: a.buffer_info()[0]  # noqa: E731
     norm = torch.empty((), dtype=torch.float32, device=device)
     nws = lib.vfd_grad_norm_workspace(n, at(numel))
     ws = _ws(nws, device)
-    args = [n, at(ptrs), at(numel), codes, int(norm_type == math.inf), *extra]
+    args = [n, at(ptrs), at(numel), _clip_codes(tensors), int(norm_type == math.inf), *extra]
     if fn == 'clip_grads':
         if outs is None:
             args += [None, None]
         else:
-            optrs = array.array('Q', [t.data_ptr() for t in outs])
-            args += [at(optrs), bytes([_CLIP_DTYPES[t.dtype] for t in outs])]
+            optrs = array.array('Q', map(torch.Tensor.data_ptr, outs))
+            args += [at(optrs), _clip_codes(outs)]
     L.check(getattr(lib, 'vfd_' + fn)(*args, norm.data_ptr(), ws.data_ptr(), nws, L.stream()), fn)
     if L.PROF_ON:                            # compulsory: the gradients once, the clipped ones once
         L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in tensors)
@@ -2352,15 +2385,18 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     if not max_norm >= 0:
         raise ValueError(f'clip_grads: max_norm must be a number >= 0, got {max_norm}')
     if out is None:
-        if not all([_dense(t) for t in tensors]):
+        if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(_dense, tensors)):
             raise ValueError('clip_grads: a gradient that is not stored densely is clipped into `out`, not in place')
         norm = _clip_call('clip_grads', tensors, norm_type, (max_norm,))
     else:
         outs = _clip_list(out, 'clip_grads out')
         if len(outs) != len(tensors):
             raise ValueError(f'clip_grads: {len(tensors)} gradients, {len(outs)} outputs')
-        work = []
-        for t, o in zip(tensors, outs):
+        work = tensors
+        if not (all(map(torch.Tensor.is_contiguous, tensors)) and all(map(torch.Tensor.is_contiguous, outs))
+                and all(map(operator.eq, map(_shape_of, tensors), map(_shape_of, outs)))):
+            work = []
+        for t, o in zip(tensors, outs) if work is not tensors else ():
             if t.shape != o.shape:
                 raise ValueError(f'clip_grads: gradient {tuple(t.shape)} into output {tuple(o.shape)}')
             if not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _dense(t)):
@@ -2370,7 +2406,8 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
             work.append(t)
         norm = _clip_call('clip_grads', work, norm_type, (max_norm,), outs)
         tensors = outs
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    torch.autograd.graph.increment_version(
+        [t for t in tensors if not t.is_inference()] if any(map(torch.Tensor.is_inference, tensors)) else tensors)
     return norm
 
 

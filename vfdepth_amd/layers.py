@@ -154,7 +154,7 @@ def layer_norm(ln, x):
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and len(ln.normalized_shape) == 1 and x.dim() >= 1
             and x.shape[-1] == ln.normalized_shape[0]):
         from . import kernels as KN
-        w, b = (None if p is None else p.float() for p in (ln.weight, ln.bias))
+        w, b = (p if p is None or p.dtype == torch.float32 else p.float() for p in (ln.weight, ln.bias))
         return KN.LayerNorm.apply(x, w, b, ln.eps)
     return ln(x)
 
