@@ -86,9 +86,9 @@ def test_workspace_counts_partials():
         a = array.array('q', numel)
         return lib.vfd_grad_norm_workspace(len(numel), a.buffer_info()[0])
     assert ws([]) == 8 and ws([0, 0]) == 8
-    assert ws([1]) == 16 and ws([4096]) == 16 and ws([4097]) == 24
+    assert ws([1]) == 16 and ws([8192]) == 16 and ws([8193]) == 24
     assert ws([1] * 177) == 8 * (177 + 1)
-    assert ws([4096 * 2049]) == 8 * (1025 + 1)            # two rounds of 1025 blocks, not 2048 and 1
+    assert ws([8192 * 2049]) == 8 * (1025 + 1)            # two rounds of 1025 blocks, not 2048 and 1
 
 
 def test_refuses_cpu_tensors_and_types():

@@ -14,7 +14,7 @@
 
 namespace vfd {
 
-constexpr int CLIP_CH = 4096;              // elements of one chunk: 16 per thread, 4 (fp32) or 2 (bf16) 16-B loads in flight
+constexpr int CLIP_CH = 8192;              // elements of one chunk: 32 per thread, 8 (fp32) or 4 (bf16) 16-B loads in flight
 constexpr int CLIP_NORM_CAP = 176;         // tensors of one launch: the table stays under 4 KB of kernel arguments
 constexpr int CLIP_SCALE_CAP = 120;
 constexpr int CLIP_GRID = 2048;            // 8 blocks per CU
@@ -97,11 +97,11 @@ __device__ __forceinline__ double norm_total(const double* __restrict__ part, in
 template <bool INF, typename T>
 __device__ __forceinline__ void norm_chunk(double& acc, const T* __restrict__ p, long long left) {
   if (left >= CLIP_CH) {
-    clip_v8<T> v[2];
+    clip_v8<T> v[CLIP_CH / 2048];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) v[u] = *reinterpret_cast<const clip_v8<T>*>(p + u * 2048 + threadIdx.x * 8);
+    for (int u = 0; u < CLIP_CH / 2048; ++u) v[u] = *reinterpret_cast<const clip_v8<T>*>(p + u * 2048 + threadIdx.x * 8);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < CLIP_CH / 2048; ++u)
 #pragma unroll
       for (int j = 0; j < 8; ++j) norm_take<INF>(acc, (float)v[u][j]);
   } else {
@@ -146,11 +146,11 @@ __global__ __launch_bounds__(256) void grad_norm_fin_k(const double* __restrict_
 template <typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const T* p, O* o, long long left, float c) {
   if (left >= CLIP_CH) {
-    clip_v8<T> v[2];
+    clip_v8<T> v[CLIP_CH / 2048];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) v[u] = *reinterpret_cast<const clip_v8<T>*>(p + u * 2048 + threadIdx.x * 8);
+    for (int u = 0; u < CLIP_CH / 2048; ++u) v[u] = *reinterpret_cast<const clip_v8<T>*>(p + u * 2048 + threadIdx.x * 8);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < CLIP_CH / 2048; ++u) {
       clip_v8<O> r;
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] = (O)((float)v[u][j] * c);
@@ -173,7 +173,8 @@ __global__ __launch_bounds__(256) void grad_scale_k(const ScaleTable t, const do
   const float c = f > 1.0 ? 1.f : (float)f;                  // NaN stays NaN: a bad gradient must not pass unseen
   if (in_place && c == 1.f) return;
   const ClipFind<CLIP_SCALE_CAP> find(t.t);
-  for (int k = blockIdx.x; k < t.t.chunks; k += gridDim.x) {
+  for (int b = blockIdx.x; b < t.t.chunks; b += gridDim.x) {
+    const int k = t.t.chunks - 1 - b;                        // backwards: what the norm read last is still cached
     const int i = find(k);
     const long long at = (long long)(k - t.t.start[i]) * CLIP_CH, left = t.t.n[i] - at;
     const void* p = t.t.p[i];
@@ -282,8 +283,8 @@ static int clip_run(int n, const void* const* grads, const int64_t* numel, const
   }
   ScaleTable t;
   int which[CLIP_SCALE_CAP];
-  for (int i = 0; i < n;) {
-    i = clip_fill(t.t, i, n, grads, numel, dt, which);
+  for (int first = (n - 1) / CLIP_SCALE_CAP * CLIP_SCALE_CAP; first >= 0; first -= CLIP_SCALE_CAP) {     // likewise
+    clip_fill(t.t, first, std::min(n, first + CLIP_SCALE_CAP), grads, numel, dt, which);
     if (t.t.chunks == 0) continue;
     for (int k = 0; k < t.t.count; ++k) {
       t.out[k] = outs ? outs[which[k]] : const_cast<void*>(t.t.p[k]);

@@ -100,6 +100,16 @@ __device__ __forceinline__ lin_f16 lin_mma(lin_f4 a, lin_f4 b, lin_f16 c) {
   return c;
 }
 
+// A chunk moved down by d >= 0 values, zeros behind it
+template <typename T>
+__device__ __forceinline__ typename LinT<T>::vec lin_down(typename LinT<T>::vec v, int d) {
+  unsigned __int128 u;
+  __builtin_memcpy(&u, &v, 16);
+  u = d >= LinT<T>::VE ? (unsigned __int128)0 : u >> (d * 8 * (int)sizeof(T));
+  __builtin_memcpy(&v, &u, 16);
+  return v;
+}
+
 // One operand of a product: element (o, k) at p[o * ld + k] (MC = false) or p[k * ld + o] (MC = true).
 template <typename T>
 struct LinOp {
@@ -131,28 +141,30 @@ struct LinTile {
   static __device__ __forceinline__ int at(int row, int c) {       // byte offset of a chunk
     return row * (CPR * 16) + ((c ^ turn(row)) << 4);
   }
+  // A tile through registers, at any alignment and with any edge: every load is unconditional and in bounds (a chunk that
+  // would leave its row starts VE before the row's end and is shifted down, zeros behind it), so that they all fly together.
   static __device__ __forceinline__ void fetch(const LinOp<T>& op, int o0, int k0, typename X::vec (&v)[NCH]) {
-    const bool whole = o0 + BO <= op.O && k0 + BK <= op.K;
+    const int len = MC ? op.O : op.K;                   // of a row in memory
+    const bool whole = k0 + BK <= op.K && (!MC || o0 + BO <= op.O);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int e = (int)threadIdx.x + i * NT;
-      const int row = e / CPR, c = e % CPR;
-      const int o = o0 + (MC ? c * X::VE : row), k = k0 + (MC ? row : c * X::VE);
-      const T* p = op.p + (MC ? (size_t)k * op.ld + o : (size_t)o * op.ld + k);
+      const int row = e / CPR, c = (e % CPR) * X::VE;
+      const int r = MC ? min(k0 + row, op.K - 1) : min(o0 + row, op.O - 1), at = (MC ? o0 : k0) + c;
+      const T* p = op.p + (size_t)r * op.ld;
       if (whole) {
-        v[i] = *reinterpret_cast<const typename X::vec*>(p);
+        v[i] = *reinterpret_cast<const typename X::vec*>(p + at);
+      } else if (len >= X::VE) {
+        const int from = min(at, len - X::VE);
+        v[i] = lin_down<T>(*reinterpret_cast<const typename X::vec*>(p + from), at - from);
       } else {
-        const int n = (o < op.O && k < op.K) ? min(MC ? op.O - o : op.K - k, X::VE) : 0;
-        if (n == X::VE) {
-          v[i] = *reinterpret_cast<const typename X::vec*>(p);
-        } else {
 #pragma unroll
-          for (int j = 0; j < X::VE; ++j) v[i][j] = (T)0.f;
-#pragma unroll
-          for (int j = 0; j < X::VE; ++j)
-            if (j < n) v[i][j] = p[j];
+        for (int j = 0; j < X::VE; ++j) {
+          const T t = p[min(at + j, len - 1)];
+          v[i][j] = at + j < len ? t : (T)0.f;
         }
       }
+      if (MC && !whole && k0 + row >= op.K) v[i] = lin_down<T>(v[i], X::VE);
     }
   }
   static __device__ __forceinline__ void put(char* lds, const typename X::vec (&v)[NCH]) {
@@ -477,6 +489,89 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// At most 16 MB rows of x (a frame's tokens): bound by reading W once, so nothing is staged.  A block owns 16 rows of W,
+// its eight waves take the contraction in turn (16 rows x 64 bytes of W a load, the x rows beside them from cache), and
+// their sums meet in LDS.
+constexpr int LIN_THIN = 64;
+__device__ __forceinline__ lin_f4 lin_mma16(lin_b8 a, lin_b8 b, lin_f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ lin_f4 lin_mma16(lin_f4 a, lin_f4 b, lin_f4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T, int MB, int ACT>
+__global__ __launch_bounds__(512) void lin_thin_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep) {
+  typedef LinT<T> X;
+  constexpr int W = 8, STEP = 4 * X::VE, U = 4;
+  __shared__ lin_f4 sm[W][MB][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = x.K, M = x.O, N = w.O;
+  const int n0 = blockIdx.x * 16, kl = (lane >> 4) * X::VE;
+  const T* pw = w.p + (size_t)min(n0 + (lane & 15), N - 1) * w.ld;
+  const T* px[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) px[i] = x.p + (size_t)min(16 * i + (lane & 15), M - 1) * x.ld;
+  lin_f4 acc[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) acc[i] = lin_f4{0.f, 0.f, 0.f, 0.f};
+  int k = wave * STEP;
+  for (; k + (U - 1) * W * STEP + STEP <= K; k += U * W * STEP) {
+    typename X::vec vw[U], vx[U][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * W * STEP + kl;
+      vw[u] = *reinterpret_cast<const typename X::vec*>(pw + at);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) vx[u][i] = *reinterpret_cast<const typename X::vec*>(px[i] + at);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) acc[i] = lin_mma16((typename X::avec)vw[u], (typename X::avec)vx[u][i], acc[i]);
+  }
+  auto edge = [&](const T* p, int at) {
+    typename X::vec v;
+    if (K >= X::VE) {
+      const int from = min(at, K - X::VE);
+      return lin_down<T>(*reinterpret_cast<const typename X::vec*>(p + from), at - from);
+    }
+#pragma unroll
+    for (int j = 0; j < X::VE; ++j) {
+      const T t = p[min(at + j, K - 1)];
+      v[j] = at + j < K ? t : (T)0.f;
+    }
+    return v;
+  };
+  for (; k < K; k += W * STEP) {
+    const typename X::vec vw = edge(pw, k + kl);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[i] = lin_mma16((typename X::avec)vw, (typename X::avec)edge(px[i], k + kl), acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i) sm[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (threadIdx.x >= 64 * MB) return;
+  // wave i finishes rows 16 i ..: a lane has row 16 i + (lane & 15), columns n0 + 4 (lane >> 4) ..
+  const int m = 16 * wave + (lane & 15), n = n0 + 4 * (lane >> 4);
+  lin_f4 v = sm[0][wave][lane];
+#pragma unroll
+  for (int r = 1; r < W; ++r) v += sm[r][wave][lane];
+  if (m >= M) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= N) continue;
+    const size_t at = (size_t)m * N + n + e;
+    float z = v[e] + (ep.bias ? ld1(ep.bias + n + e) : 0.f);
+    if (ep.z) st1(ep.z + at, z);
+    z = lin_act<ACT>(z);
+    if (ep.res) z += ld1(ep.res + at);
+    st1(ep.y + at, z);
+  }
+}
+
 // A split contraction's partial products, added in split order, and the epilogue.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int M, int N) {
@@ -520,28 +615,52 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-  if (cnt > 0)
-    for (long long m = (long long)blockIdx.y * 4 + wave; m < M; m += (long long)gridDim.y * 4) {
-      const size_t at = (size_t)m * N + n;
-      vec gv, zv, o;
-      if (cnt == V) {
-        gv = *reinterpret_cast<const vec*>(g + at);
-        if (ACT != LIN_NONE) zv = *reinterpret_cast<const vec*>(z + at);
-      } else {
+  if (cnt > 0) {
+    constexpr int U = 2;                                   // rows in flight a lane, and as many more being fetched
+    const long long step = (long long)gridDim.y * 4;
+    vec gv[U], zv[U];
+    auto fetch = [&](long long m) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          gv[j] = j < cnt ? g[at + j] : (T)0.f;
-          if (ACT != LIN_NONE) zv[j] = j < cnt ? z[at + j] : (T)0.f;
+      for (int u = 0; u < U; ++u) {
+        const size_t at = (size_t)min(m + u * step, (long long)M - 1) * N + n;
+        if (cnt == V) {
+          gv[u] = *reinterpret_cast<const vec*>(g + at);
+          if (ACT != LIN_NONE) zv[u] = *reinterpret_cast<const vec*>(z + at);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            gv[u][j] = j < cnt ? g[at + j] : (T)0.f;
+            if (ACT != LIN_NONE) zv[u][j] = j < cnt ? z[at + j] : (T)0.f;
+          }
         }
       }
+    };
+    long long m = (long long)blockIdx.y * 4 + wave;
+    if (m < M) fetch(m);
+    while (m < M) {
+      float f[U][V], zf[U][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float f = (float)gv[j];
-        if (ACT != LIN_NONE) f *= lin_slope<ACT>((float)zv[j]);
-        s[j] += f;
-        o[j] = (T)f;
-      }
-      if (ACT != LIN_NONE) {
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          f[u][j] = (float)gv[u][j];
+          if (ACT != LIN_NONE) zf[u][j] = (float)zv[u][j];
+        }
+      const long long m0 = m;
+      m += U * step;
+      if (m < M) fetch(m);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (m0 + u * step >= M) continue;
+        vec o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (ACT != LIN_NONE) f[u][j] *= lin_slope<ACT>(zf[u][j]);
+          s[j] += f[u][j];
+          o[j] = (T)f[u][j];
+        }
+        if (ACT == LIN_NONE) continue;
+        const size_t at = (size_t)(m0 + u * step) * N + n;
         if (cnt == V) {
           *reinterpret_cast<vec*>(gz + at) = o;
         } else {
@@ -551,6 +670,7 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
         }
       }
     }
+  }
   if (part == nullptr) return;
 #pragma unroll
   for (int j = 0; j < V; ++j) sm[wave][lane][j] = s[j];
@@ -564,7 +684,6 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
 
 // ---------------------------------------------------------------- host
 constexpr int LIN_CUS = 256;
-constexpr int LIN_RB = 128, LIN_SLOTS = 2;   // rings of four or five tiles of 64 bytes: 3 to 20 % slower (16 384 x 2048 x 8192)
 
 struct LinPlan {
   int tm, tn, splits;
@@ -622,18 +741,63 @@ static bool lin_aligned(const LinOp<T>& op) {
   return ((uintptr_t)op.p & 15) == 0 && op.ld % VE == 0 && (!MC || op.O % VE == 0) && op.ld < (1 << 20);
 }
 
-// bf16 products with enough 256 x 256 tiles to fill the chip take them (half the LDS reads a product of 128 x 128 tiles)
+// Which tiles a bf16 product takes.  Both measured with their contraction's length (one box, microseconds): a round of 256
+// tiles of 256 x 256 (one a CU, 8 waves) takes 1.6 per 64 contraction values and 9 to start and to store; a round of 512
+// tiles of 128 x 128 (two a CU, 4 waves each) 0.95 and 2.1: 8192^3 819 against 970, 16 384 x 2048 x 8192 483 against 518,
+// but 92 160 x 256 x 1024 101 against 65 (forward), 23 040 x 1024 x 256 33 against 28.
 template <typename T>
-static bool lin_big(int M, int N) {
-  return sizeof(T) == 2 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= LIN_CUS;
+static bool lin_big(int M, int N, int K) {
+  if (sizeof(T) != 2) return false;
+  const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256), t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
+  const double kt = K / 64.0;
+  const double big = (double)((t256 + LIN_CUS - 1) / LIN_CUS) * (1.6 * kt + 9.0);
+  const double half_rounds = (double)((t128 + LIN_CUS - 1) / LIN_CUS);
+  return t256 * 2 > LIN_CUS && big < (half_rounds < 2 ? 2 : half_rounds) * 0.5 * (0.95 * kt + 2.1);
+}
+
+// 128 x 128 tiles through three 64-byte slots, three blocks a CU, where a block is short (its loads, products and stores
+// then overlap another's), or through two 128-byte slots, two blocks a CU.  Measured (microseconds, short / long slots):
+// forward 92 160 x 256 x 64 bf16 18 / 22, 23 040 x 256 x 1024 fp32 107 / 114, but 8192 x 2048 x 2048 fp32 588 / 486; data
+// gradient at a contraction of 256 97 / 117, of 1024 29 / 24; weight gradient (both operands read across) 95 / 76.
+template <bool XMC>
+static bool lin_short(int K) {
+  return !XMC && K <= 512;
+}
+
+// fp32 products are bound by the matrix cores alone: 64-row tiles where 128-row ones leave the last round emptier (by more
+// than the tenth that the smaller tiles cost)
+template <typename T>
+static bool lin_flat(int M, int N) {
+  if (sizeof(T) != 4) return false;
+  const long long tn = (N + 127) / 128, half = ((M + 63) / 64 * tn + LIN_CUS - 1) / LIN_CUS, full = ((M + 127) / 128 * tn + LIN_CUS - 1) / LIN_CUS;
+  return full > 1 && half * 11 <= full * 20;
+}
+
+enum LinForm { LIN_F_BIG, LIN_F_FLAT, LIN_F_SHORT, LIN_F_LONG };
+struct LinChoice {
+  LinForm form;
+  LinPlan plan;
+};
+template <typename T, bool XMC, bool WMC>
+static LinChoice lin_choose(int M, int N, int K, bool aligned) {
+  if (aligned && lin_big<T>(M, N, K)) return {LIN_F_BIG, LinPlan{(M + 255) / 256, (N + 255) / 256, 1}};
+  if (aligned && lin_flat<T>(M, N)) return {LIN_F_FLAT, LinPlan{(M + 63) / 64, (N + 127) / 128, 1}};
+  if (lin_short<XMC>(K)) return {LIN_F_SHORT, lin_plan<T, 128, 128>(M, N, K, 3)};
+  return {LIN_F_LONG, lin_plan<T, 128, 128>(M, N, K, 2)};
 }
 
 template <typename T, bool XMC, bool WMC, bool ASYNC>
 static int lin_sized(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, float* part, hipStream_t s) {
-  if constexpr (sizeof(T) == 2 && ASYNC)
-    if (lin_big<T>(x.O, w.O))
-      return lin_launch<T, XMC, WMC, 256, 256, 2, 2, 1, LIN_RB, LIN_SLOTS, ASYNC>(x, w, ep, lin_plan<T, 256, 256>(x.O, w.O, x.K, 1), part, s);
-  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, LIN_RB, LIN_SLOTS, ASYNC>(x, w, ep, lin_plan<T, 128, 128>(x.O, w.O, x.K, 2), part, s);
+  const LinChoice c = lin_choose<T, XMC, WMC>(x.O, w.O, x.K, ASYNC);
+  if constexpr (ASYNC) {
+    if constexpr (sizeof(T) == 2)
+      if (c.form == LIN_F_BIG) return lin_launch<T, XMC, WMC, 256, 256, 2, 4, 2, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
+    if constexpr (sizeof(T) == 4)
+      if (c.form == LIN_F_FLAT) return lin_launch<T, XMC, WMC, 64, 128, 2, 2, 3, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
+  }
+  if constexpr (!XMC)
+    if (c.form == LIN_F_SHORT) return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 3, 64, 3, ASYNC>(x, w, ep, c.plan, part, s);
+  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
 }
 
 template <typename T, bool XMC, bool WMC>
@@ -642,10 +806,12 @@ static int lin_product(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep
   return lin_sized<T, XMC, WMC, false>(x, w, ep, part, s);
 }
 
-template <typename T>
+// Of whichever of the two forms (by alignment, which a descriptor does not say) needs more
+template <typename T, bool XMC, bool WMC>
 static size_t lin_part_bytes(int M, int N, int K) {
-  const LinPlan p = lin_plan<T, 128, 128>(M, N, K, 2);
-  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  const int a = lin_choose<T, XMC, WMC>(M, N, K, true).plan.splits, b = lin_choose<T, XMC, WMC>(M, N, K, false).plan.splits;
+  const int splits = a > b ? a : b;
+  return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
 }
 
 static int lin_strips(int M, int N, int V) {               // row blocks of lin_act_bwd_k
@@ -653,12 +819,14 @@ static int lin_strips(int M, int N, int V) {               // row blocks of lin_
   return need < most ? need : most;
 }
 
+static bool lin_is_thin(const vfd_linear_desc* d) { return d->rows <= LIN_THIN && d->k > 0; }
+
 template <typename T>
 static size_t lin_ws(const vfd_linear_desc* d, int what) {
   switch (what) {
-    case VFD_LINEAR_FWD: return lin_part_bytes<T>(d->rows, d->n, d->k);
-    case VFD_LINEAR_DGRAD: return lin_part_bytes<T>(d->rows, d->k, d->n);
-    case VFD_LINEAR_WGRAD: return lin_part_bytes<T>(d->n, d->k, d->rows);
+    case VFD_LINEAR_FWD: return lin_is_thin(d) ? 0 : lin_part_bytes<T, false, false>(d->rows, d->n, d->k);
+    case VFD_LINEAR_DGRAD: return lin_part_bytes<T, false, true>(d->rows, d->k, d->n);
+    case VFD_LINEAR_WGRAD: return lin_part_bytes<T, true, true>(d->n, d->k, d->rows);
     case VFD_LINEAR_ACT_BWD: return (size_t)lin_strips(d->rows, d->n, LinT<T>::VE) * d->n * sizeof(float);
   }
   return 0;
@@ -680,6 +848,16 @@ static int lin_fwd_run(const vfd_linear_desc* d, const void* x, const void* w, c
                        void* z, float* part, hipStream_t s) {
   const LinOp<T> ox{(const T*)x, d->ldx, d->rows, d->k}, ow{(const T*)w, d->k, d->n, d->k};
   const LinEpi<T> ep{(const T*)bias, (const T*)res, (T*)z, (T*)y, nullptr, d->act};
+  if (lin_is_thin(d)) {
+    lin_with_act(d->act, [&](auto act) {
+      const unsigned grid = (unsigned)((d->n + 15) / 16);
+      if (d->rows <= 16) lin_thin_k<T, 1, act()><<<grid, 512, 0, s>>>(ox, ow, ep);
+      else if (d->rows <= 32) lin_thin_k<T, 2, act()><<<grid, 512, 0, s>>>(ox, ow, ep);
+      else lin_thin_k<T, 4, act()><<<grid, 512, 0, s>>>(ox, ow, ep);
+      return 0;
+    });
+    return fail_launch("linear_fwd");
+  }
   return lin_product<T, false, false>(ox, ow, ep, part, s);
 }
 

@@ -2315,18 +2315,17 @@ def _clip_list(tensors, what):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     # whole-list passes (a model has hundreds of gradients, and the kernels take tens of microseconds), tensor by tensor
     # only to name the one that does not fit
-    if all(map(torch.is_tensor, tensors)) and not set(map(torch.Tensor.get_device, tensors)) - {_current_device(tensors)} \
-            and set(map(_dtype_of, tensors)) <= _CLIP_DTYPES.keys() and set(map(_layout_of, tensors)) <= {torch.strided}:
-        return tensors
+    try:
+        if (set(map(torch.Tensor.get_device, tensors)) <= {torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None}
+                and set(map(_dtype_of, tensors)) <= _CLIP_DTYPES.keys() and set(map(_layout_of, tensors)) <= {torch.strided}):
+            return tensors
+    except TypeError:                       # something that is no tensor
+        pass
     for t in tensors:
         _check_device(t, what)
         if t.dtype not in _CLIP_DTYPES or t.layout is not torch.strided:
             raise RuntimeError(f'{what}: strided fp32 or bf16 tensors, got {t.dtype} ({t.layout})')
     return tensors
-
-
-def _current_device(tensors):
-    return torch._C._cuda_getDevice() if any(t.is_cuda for t in tensors[:1]) else None
 
 
 def _clip_codes(tensors):
@@ -2406,8 +2405,10 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
             work.append(t)
         norm = _clip_call('clip_grads', work, norm_type, (max_norm,), outs)
         tensors = outs
-    torch.autograd.graph.increment_version(
-        [t for t in tensors if not t.is_inference()] if any(map(torch.Tensor.is_inference, tensors)) else tensors)
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                    # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
     return norm
 
 
