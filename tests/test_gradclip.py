@@ -15,7 +15,7 @@ HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8}
 
 
 def _sizes(kind):
-    return {'one': [1], 'tail': [4095, 4096, 4097, 1, 3], 'empty': [0, 7, 0, 4096, 0],
+    return {'one': [1], 'tail': [16383, 16384, 16385, 4096, 1, 3], 'empty': [0, 7, 0, 16384, 0],
             'many': [(i * 37) % 511 + 1 for i in range(400)], 'large': [3_000_001, 5, 1_048_576]}[kind]
 
 
@@ -86,9 +86,9 @@ def test_workspace_counts_partials():
         a = array.array('q', numel)
         return lib.vfd_grad_norm_workspace(len(numel), a.buffer_info()[0])
     assert ws([]) == 8 and ws([0, 0]) == 8
-    assert ws([1]) == 16 and ws([8192]) == 16 and ws([8193]) == 24
+    assert ws([1]) == 16 and ws([16384]) == 16 and ws([16385]) == 24
     assert ws([1] * 177) == 8 * (177 + 1)
-    assert ws([8192 * 2049]) == 8 * (1025 + 1)            # two rounds of 1025 blocks, not 2048 and 1
+    assert ws([16384 * 2049]) == 8 * (1025 + 1)            # two rounds of 1025 blocks, not 2048 and 1
 
 
 def test_refuses_cpu_tensors_and_types():

@@ -14,7 +14,7 @@
 
 namespace vfd {
 
-constexpr int CLIP_CH = 8192;              // elements of one chunk: 32 per thread, 8 (fp32) or 4 (bf16) 16-B loads in flight
+constexpr int CLIP_CH = 16384;             // elements of one chunk: 64 per thread, 16 (fp32) or 8 (bf16) 16-B loads in flight
 constexpr int CLIP_NORM_CAP = 176;         // tensors of one launch: the table stays under 4 KB of kernel arguments
 constexpr int CLIP_SCALE_CAP = 120;
 constexpr int CLIP_GRID = 2048;            // 8 blocks per CU

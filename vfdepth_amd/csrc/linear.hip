@@ -815,7 +815,7 @@ static size_t lin_part_bytes(int M, int N, int K) {
 }
 
 static int lin_strips(int M, int N, int V) {               // row blocks of lin_act_bwd_k
-  const int cb = (N + 64 * V - 1) / (64 * V), most = 2048 / cb > 0 ? 2048 / cb : 1, need = (M + 15) / 16;
+  const int cb = (N + 64 * V - 1) / (64 * V), most = 4096 / cb > 0 ? 4096 / cb : 1, need = (M + 15) / 16;
   return need < most ? need : most;
 }
 

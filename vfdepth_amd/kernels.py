@@ -2175,10 +2175,10 @@ class LayerNorm(torch.autograd.Function):
         d = L.NormDesc(rows, C, ldx, eps, code)
         weight = weight.contiguous() if weight is not None else None
         bias = bias.contiguous() if bias is not None else None
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         stats = m = r = None
         if any(ctx.needs_input_grad):
-            stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)      # means, then 1 / deviations
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=y.device)      # means, then 1 / deviations
             m = stats.data_ptr()
             r = m + 4 * rows
         L.check(lib.vfd_layer_norm_fwd(ctypes.byref(d), x2.data_ptr(), L.ptr(weight), L.ptr(bias), y.data_ptr(), m, r,
@@ -2197,8 +2197,8 @@ class LayerNorm(torch.autograd.Function):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         g = _as(g, x)
         dx = torch.empty_like(g) if need_x else None
-        dw = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need_w else None
-        db = torch.empty(d.cols, dtype=torch.float32, device=x.device) if need_b else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = (torch.empty(d.cols, dtype=torch.float32, device=g.device) if weight is None else torch.empty_like(weight)) if need_b else None
         ws, nws = None, 0
         if need_w or need_b:
             nws = lib.vfd_layer_norm_bwd_workspace(ctypes.byref(d))
