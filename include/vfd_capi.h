@@ -599,27 +599,21 @@ int vfd_layer_norm_bwd(const vfd_norm_desc* d, const void* g, const void* x, con
 /* ------------------------------------------------------------------ linear layer with epilogue */
 #define VFD_LINEAR_MAX (1 << 30)
 typedef struct vfd_linear_desc {
-  int32_t rows, k, n;    /* x [rows, k], w [n, k], y [rows, n]; each 0 .. VFD_LINEAR_MAX            */
+  int32_t rows, k, n;    /* x [rows, k], w [n, k], y [rows, n]; at most VFD_LINEAR_MAX, k and n at least 1 */
   int32_t act;           /* 0 none, 1 ReLU, 2 LeakyReLU(0.1), 3 ELU, 4 GELU (erf), 5 SiLU           */
   int64_t ldx;           /* elements from one row of x to the next (>= k); all others are dense     */
   int32_t dtype;         /* of every tensor: 0 fp32, 1 bf16 (sums fp32, outputs rounded once)       */
 } vfd_linear_desc;
-enum { VFD_LINEAR_FWD = 0, VFD_LINEAR_DGRAD = 1, VFD_LINEAR_WGRAD = 2, VFD_LINEAR_ACT_BWD = 3 };
 
-/* Workspace bytes of one of the calls below (0 = none needed). */
-size_t vfd_linear_workspace(const vfd_linear_desc* d, int what);
 /* y = act(x w^T + bias) + res; bias [n], res [rows, n] and z (the pre-activation, kept for the backward) may be null. */
+size_t vfd_linear_fwd_workspace(const vfd_linear_desc* d);
 int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z,
                    void* workspace, size_t ws_bytes, void* stream);
-/* gz = g act'(z) [rows, n] (act 0: gz is g, z and gz are not used) and db [n] = its column sums (null: not computed). */
-int vfd_linear_act_bwd(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, void* workspace,
-                       size_t ws_bytes, void* stream);
-/* dx [rows, k] = gz w */
-int vfd_linear_dgrad(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, void* workspace, size_t ws_bytes,
-                     void* stream);
-/* dw [n, k] = gz^T x */
-int vfd_linear_wgrad(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, void* workspace, size_t ws_bytes,
-                     void* stream);
+/* From g [rows, n]: gz = g act'(z) (act 0: gz is g, z and gz are not used), dx [rows, k] = gz w, dw [n, k] = gz^T x and
+ * db [n] = gz's column sums; dx, dw, db null = not computed.  Fixed-order sums. */
+size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d);
+int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
+                   void* dw, void* db, void* workspace, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------ gradient norm / clipping */
 /* Global norm of n gradient tensors (grads[i]: device pointer of numel[i] densely stored elements at any element

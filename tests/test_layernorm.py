@@ -256,8 +256,8 @@ def test_refusals():
     from vfdepth_amd import kernels as KN
     x = torch.randn(4, 8, device='cuda')
     w = torch.ones(8, device='cuda')
-    for args, word in (((x.half(), w, None), 'fp32 or bf16'), ((x, w[:7], None), r'fp32 \[8\]'),
-                       ((x, w.to(BF16), None), r'fp32 \[8\]'), ((x, w, w.view(2, 4)), r'fp32 \[8\]'),
+    for args, word in (((x.half(), w, None), 'fp32 or bf16'), ((x, w[:7], None), r'float32 \[8\]'),
+                       ((x, w.to(BF16), None), r'float32 \[8\]'), ((x, w, w.view(2, 4)), r'float32 \[8\]'),
                        ((x, w.cpu(), None), 'HIP device'), ((x.cpu(), w, None), 'HIP device')):
         with pytest.raises(RuntimeError, match=word):
             KN.LayerNorm.apply(*args, EPS)

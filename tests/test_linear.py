@@ -97,7 +97,7 @@ def _desc(rows=4, k=8, n=8, act=0, ldx=8, dtype=0):
     return _lib.LinearDesc(rows, k, n, act, ldx, dtype)
 
 
-@pytest.mark.parametrize('bad', [dict(rows=-1), dict(k=-1), dict(n=-2), dict(act=6), dict(act=-1), dict(ldx=7), dict(dtype=2),
+@pytest.mark.parametrize('bad', [dict(rows=-1), dict(k=0, ldx=0), dict(n=0), dict(n=-2), dict(act=6), dict(act=-1), dict(ldx=7), dict(dtype=2),
                                  dict(rows=(1 << 30) + 1), dict(rows=1 << 30, n=1 << 30)])
 def test_c_refuses_bad_descriptors(bad):
     from vfdepth_amd import _lib
@@ -105,32 +105,32 @@ def test_c_refuses_bad_descriptors(bad):
     d = _desc(**bad)
     p = 1 << 40
     for rc in (lib.vfd_linear_fwd(ctypes.byref(d), p, p, p, p, p, p, p, 1 << 40, None),
-               lib.vfd_linear_act_bwd(ctypes.byref(d), p, p, p, p, p, 1 << 40, None),
-               lib.vfd_linear_dgrad(ctypes.byref(d), p, p, p, p, 1 << 40, None),
-               lib.vfd_linear_wgrad(ctypes.byref(d), p, p, p, p, 1 << 40, None)):
+               lib.vfd_linear_bwd(ctypes.byref(d), p, p, p, p, p, p, p, p, p, 1 << 40, None)):
         assert rc == -1 and (b'descriptor' in lib.vfd_last_error() or b'tiles' in lib.vfd_last_error())
-    assert lib.vfd_linear_workspace(ctypes.byref(d), 0) == 0
+    assert lib.vfd_linear_fwd_workspace(ctypes.byref(d)) == lib.vfd_linear_bwd_workspace(ctypes.byref(d)) == 0
 
 
 def test_c_refuses_null_tensors_and_small_workspaces():
     from vfdepth_amd import _lib
     lib = _lib.load()
-    p = 1 << 40
+    p, no = 1 << 40, None
     d = _desc()
-    assert lib.vfd_linear_fwd(ctypes.byref(d), None, p, None, None, p, None, p, 1 << 40, None) == -1
-    assert lib.vfd_linear_fwd(ctypes.byref(d), p, p, None, None, None, None, p, 1 << 40, None) == -1
-    assert lib.vfd_linear_dgrad(ctypes.byref(d), p, None, p, p, 1 << 40, None) == -1
-    assert lib.vfd_linear_wgrad(ctypes.byref(d), p, p, None, p, 1 << 40, None) == -1
+
+    def bwd(g=p, z=no, w=p, x=p, gz=no, dx=p, dw=p, db=p, ws=p, n=1 << 40):
+        return lib.vfd_linear_bwd(ctypes.byref(d), g, z, w, x, gz, dx, dw, db, ws, n, no)
+    assert lib.vfd_linear_fwd(ctypes.byref(d), no, p, no, no, p, no, p, 1 << 40, no) == -1
+    assert lib.vfd_linear_fwd(ctypes.byref(d), p, p, no, no, no, no, p, 1 << 40, no) == -1
+    assert bwd(g=no) == bwd(w=no) == bwd(x=no) == bwd(ws=no) == -1
+    assert bwd(dx=no, dw=no, db=no) == 0                                         # nothing asked for: nothing is launched
     d = _desc(act=4)
-    assert lib.vfd_linear_act_bwd(ctypes.byref(d), p, None, p, p, p, 1 << 40, None) == -1
+    assert bwd(gz=p) == bwd(z=p) == -1 and b'null' in lib.vfd_last_error()
     d = _desc(rows=100000, k=128, n=128, ldx=128)
-    need = lib.vfd_linear_workspace(ctypes.byref(d), _lib.LINEAR_WGRAD)
-    assert need > 0 and lib.vfd_linear_wgrad(ctypes.byref(d), p, p, p, p, need - 1, None) == -1
-    assert b'workspace' in lib.vfd_last_error()
-    need = lib.vfd_linear_workspace(ctypes.byref(d), _lib.LINEAR_ACT_BWD)
-    assert need > 0 and lib.vfd_linear_act_bwd(ctypes.byref(d), p, p, p, p, p, need - 1, None) == -1
-    for d in (_desc(rows=0), _desc(n=0)):                                        # nothing to do: nothing is launched
-        assert lib.vfd_linear_fwd(ctypes.byref(d), *[None] * 7, 0, None) == 0
+    need = lib.vfd_linear_bwd_workspace(ctypes.byref(d))
+    assert need > 0 and bwd(n=need - 1) == -1 and b'workspace' in lib.vfd_last_error()
+    d = _desc(rows=300, k=8192, n=128, ldx=8192)                                 # few tiles: the contraction is split
+    need = lib.vfd_linear_fwd_workspace(ctypes.byref(d))
+    assert need > 0 and lib.vfd_linear_fwd(ctypes.byref(d), p, p, no, no, p, no, p, need - 1, no) == -1
+    assert lib.vfd_linear_fwd(ctypes.byref(_desc(rows=0)), *[no] * 7, 0, no) == 0
 
 
 def test_descriptor_layout(tmp_path):

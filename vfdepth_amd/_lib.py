@@ -60,8 +60,7 @@ class LinearDesc(ctypes.Structure):
     _fields_ = [('rows', c_int), ('k', c_int), ('n', c_int), ('act', c_int), ('ldx', ctypes.c_int64), ('dtype', c_int)]
 
 
-# vfd_linear_workspace's calls and vfd_linear_desc.act
-LINEAR_FWD, LINEAR_DGRAD, LINEAR_WGRAD, LINEAR_ACT_BWD = range(4)
+# vfd_linear_desc.act
 LINEAR_ACTS = {'none': 0, 'relu': 1, 'lrelu': 2, 'elu': 3, 'gelu': 4, 'silu': 5}
 
 _SIGS = {
@@ -174,11 +173,10 @@ _SIGS = {
     'vfd_layer_norm_fwd': (c_int, [ctypes.POINTER(NormDesc)] + [c_fp] * 6 + [c_void_p]),
     'vfd_layer_norm_bwd_workspace': (c_size_t, [ctypes.POINTER(NormDesc)]),
     'vfd_layer_norm_bwd': (c_int, [ctypes.POINTER(NormDesc)] + [c_fp] * 9 + [c_size_t, c_void_p]),
-    'vfd_linear_workspace': (c_size_t, [ctypes.POINTER(LinearDesc), c_int]),
+    'vfd_linear_fwd_workspace': (c_size_t, [ctypes.POINTER(LinearDesc)]),
     'vfd_linear_fwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 7 + [c_size_t, c_void_p]),
-    'vfd_linear_act_bwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 5 + [c_size_t, c_void_p]),
-    'vfd_linear_dgrad': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 4 + [c_size_t, c_void_p]),
-    'vfd_linear_wgrad': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 4 + [c_size_t, c_void_p]),
+    'vfd_linear_bwd_workspace': (c_size_t, [ctypes.POINTER(LinearDesc)]),
+    'vfd_linear_bwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 9 + [c_size_t, c_void_p]),
     'vfd_grad_norm_workspace': (c_size_t, [c_int, c_fp]),
     'vfd_grad_norm': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_fp, c_fp, c_size_t, c_void_p]),
     'vfd_clip_grads': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_double] + [c_fp] * 4 + [c_size_t, c_void_p]),

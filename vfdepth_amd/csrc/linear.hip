@@ -7,6 +7,7 @@
 // One tile kernel serves the three products: an operand is read as [outer][contraction] (its contraction contiguous:
 // x, W and gz forward) or as [contraction][outer] (W and gz, x in the gradients), and leaves LDS in the matrix
 // instructions' order either way, so nothing is transposed in memory.
+#include <algorithm>
 #include <type_traits>
 
 #include "vfd_common.h"
@@ -819,21 +820,23 @@ static int lin_strips(int M, int N, int V) {               // row blocks of lin_
   return need < most ? need : most;
 }
 
-static bool lin_is_thin(const vfd_linear_desc* d) { return d->rows <= LIN_THIN && d->k > 0; }
+static bool lin_is_thin(const vfd_linear_desc* d) { return d->rows <= LIN_THIN; }
 
 template <typename T>
-static size_t lin_ws(const vfd_linear_desc* d, int what) {
-  switch (what) {
-    case VFD_LINEAR_FWD: return lin_is_thin(d) ? 0 : lin_part_bytes<T, false, false>(d->rows, d->n, d->k);
-    case VFD_LINEAR_DGRAD: return lin_part_bytes<T, false, true>(d->rows, d->k, d->n);
-    case VFD_LINEAR_WGRAD: return lin_part_bytes<T, true, true>(d->n, d->k, d->rows);
-    case VFD_LINEAR_ACT_BWD: return (size_t)lin_strips(d->rows, d->n, LinT<T>::VE) * d->n * sizeof(float);
-  }
-  return 0;
+static size_t lin_fwd_ws(const vfd_linear_desc* d) {
+  return lin_is_thin(d) ? 0 : lin_part_bytes<T, false, false>(d->rows, d->n, d->k);
+}
+
+// The backward's steps follow each other on one stream through one workspace
+template <typename T>
+static size_t lin_bwd_ws(const vfd_linear_desc* d) {
+  const size_t act = (size_t)lin_strips(d->rows, d->n, LinT<T>::VE) * d->n * sizeof(float);
+  const size_t dx = lin_part_bytes<T, false, true>(d->rows, d->k, d->n), dw = lin_part_bytes<T, true, true>(d->n, d->k, d->rows);
+  return std::max(act, std::max(dx, dw));
 }
 
 static int lin_check(const char* what, const vfd_linear_desc* d) {
-  VFD_REQUIRE(d && d->rows >= 0 && d->k >= 0 && d->n >= 0 && d->rows <= VFD_LINEAR_MAX && d->k <= VFD_LINEAR_MAX &&
+  VFD_REQUIRE(d && d->rows >= 0 && d->k >= 1 && d->n >= 1 && d->rows <= VFD_LINEAR_MAX && d->k <= VFD_LINEAR_MAX &&
                   d->n <= VFD_LINEAR_MAX && d->ldx >= d->k && d->act >= 0 && d->act < LIN_ACTS && (d->dtype == 0 || d->dtype == 1),
               "%s: bad descriptor", what);
   const long long T = 128;
@@ -884,7 +887,18 @@ static int lin_act_bwd_run(const vfd_linear_desc* d, const void* g, const void* 
     return 0;
   });
   if (db) col_sums_k<T><<<cdiv(d->n, COLSUM_COLS), 1024, 0, s>>>(part, strips, d->n, d->n, (T*)db, nullptr);
-  return fail_launch("linear_act_bwd");
+  return fail_launch("linear_bwd activation");
+}
+
+template <typename T>
+static int lin_bwd_run(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
+                       void* dw, void* db, float* ws, hipStream_t s) {
+  if (d->act != LIN_NONE || db)
+    if (int e = lin_act_bwd_run<T>(d, g, z, gz, db, ws, s)) return e;
+  if (d->act == LIN_NONE) gz = const_cast<void*>(g);
+  if (dx)
+    if (int e = lin_dgrad_run<T>(d, gz, w, dx, ws, s)) return e;
+  return dw ? lin_wgrad_run<T>(d, gz, x, dw, ws, s) : VFD_OK;
 }
 
 }  // namespace vfd
@@ -893,62 +907,43 @@ using namespace vfd;
 
 extern "C" {
 
-size_t vfd_linear_workspace(const vfd_linear_desc* d, int what) {
-  if (lin_check("linear", d) != VFD_OK || d->rows == 0 || d->k == 0 || d->n == 0) return 0;
-  return d->dtype ? lin_ws<__bf16>(d, what) : lin_ws<float>(d, what);
+size_t vfd_linear_fwd_workspace(const vfd_linear_desc* d) {
+  if (lin_check("linear", d) != VFD_OK || d->rows == 0) return 0;
+  return d->dtype ? lin_fwd_ws<__bf16>(d) : lin_fwd_ws<float>(d);
 }
 
 int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z,
                    void* workspace, size_t ws_bytes, void* stream) {
   if (int e = lin_check("linear_fwd", d)) return e;
-  if (d->rows == 0 || d->n == 0) return VFD_OK;
-  VFD_REQUIRE(y && (d->k == 0 || (x && w)), "linear_fwd: null tensor");
-  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_FWD);
+  if (d->rows == 0) return VFD_OK;
+  VFD_REQUIRE(y && x && w, "linear_fwd: null tensor");
+  const size_t need = vfd_linear_fwd_workspace(d);
   VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_fwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof(K_LINEAR_FWD, s);
   return (d->dtype ? lin_fwd_run<__bf16> : lin_fwd_run<float>)(d, x, w, bias, res, y, z, (float*)workspace, s);
 }
 
-int vfd_linear_act_bwd(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, void* workspace,
-                       size_t ws_bytes, void* stream) {
-  if (int e = lin_check("linear_act_bwd", d)) return e;
+size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d) {
+  if (lin_check("linear", d) != VFD_OK || d->rows == 0) return 0;
+  return d->dtype ? lin_bwd_ws<__bf16>(d) : lin_bwd_ws<float>(d);
+}
+
+int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
+                   void* dw, void* db, void* workspace, size_t ws_bytes, void* stream) {
+  if (int e = lin_check("linear_bwd", d)) return e;
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof(K_LINEAR_BWD, s);
-  if (d->n == 0) return VFD_OK;
+  const size_t es = d->dtype ? 2 : 4;
   if (d->rows == 0) {
-    if (db) zero_async(db, (size_t)d->n * (d->dtype ? 2 : 4), s);
-    return fail_launch("linear_act_bwd");
+    if (dw) zero_async(dw, (size_t)d->n * d->k * es, s);
+    if (db) zero_async(db, (size_t)d->n * es, s);
+    return fail_launch("linear_bwd");
   }
-  VFD_REQUIRE(g && (d->act == LIN_NONE || (z && gz)), "linear_act_bwd: null tensor");
-  if (d->act == LIN_NONE && !db) return VFD_OK;
-  const size_t need = (size_t)lin_strips(d->rows, d->n, d->dtype ? 8 : 4) * d->n * sizeof(float);
-  VFD_REQUIRE(!db || (workspace && ws_bytes >= need), "linear_act_bwd: workspace too small");
-  return (d->dtype ? lin_act_bwd_run<__bf16> : lin_act_bwd_run<float>)(d, g, z, gz, db, (float*)workspace, s);
-}
-
-int vfd_linear_dgrad(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, void* workspace, size_t ws_bytes,
-                     void* stream) {
-  if (int e = lin_check("linear_dgrad", d)) return e;
-  if (d->rows == 0 || d->k == 0) return VFD_OK;
-  VFD_REQUIRE(dx && (d->n == 0 || (gz && w)), "linear_dgrad: null tensor");
-  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_DGRAD);
-  VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_dgrad: workspace too small");
-  hipStream_t s = (hipStream_t)stream;
-  ProfScope prof(K_LINEAR_BWD, s);
-  return (d->dtype ? lin_dgrad_run<__bf16> : lin_dgrad_run<float>)(d, gz, w, dx, (float*)workspace, s);
-}
-
-int vfd_linear_wgrad(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, void* workspace, size_t ws_bytes,
-                     void* stream) {
-  if (int e = lin_check("linear_wgrad", d)) return e;
-  if (d->k == 0 || d->n == 0) return VFD_OK;
-  VFD_REQUIRE(dw && (d->rows == 0 || (gz && x)), "linear_wgrad: null tensor");
-  const size_t need = vfd_linear_workspace(d, VFD_LINEAR_WGRAD);
-  VFD_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "linear_wgrad: workspace too small");
-  hipStream_t s = (hipStream_t)stream;
-  ProfScope prof(K_LINEAR_BWD, s);
-  return (d->dtype ? lin_wgrad_run<__bf16> : lin_wgrad_run<float>)(d, gz, x, dw, (float*)workspace, s);
+  if (!dx && !dw && !db) return VFD_OK;
+  VFD_REQUIRE(g && (d->act == LIN_NONE || (z && gz)) && (!dx || w) && (!dw || x), "linear_bwd: null tensor");
+  VFD_REQUIRE(workspace && ws_bytes >= vfd_linear_bwd_workspace(d), "linear_bwd: workspace too small");
+  return (d->dtype ? lin_bwd_run<__bf16> : lin_bwd_run<float>)(d, g, z, w, x, gz, dx, dw, db, (float*)workspace, s);
 }
 
 }  // extern "C"

@@ -2148,6 +2148,15 @@ def _once(fn):
     return staticmethod(backward)
 
 
+def _param(t, x, dtype, shape, what):
+    """A further operand of x's operator, dense: on x's device, of this type and shape."""
+    if not torch.is_tensor(t) or t.get_device() != x.get_device():
+        _check_device(t, what)
+    if t.dtype != dtype or t.shape != shape:
+        raise RuntimeError(f'{what}: {str(dtype)[6:]} {list(shape)}, got {str(t.dtype)[6:]} {list(t.shape)}')
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _as(t, like):
     """An incoming gradient, dense and of the forward's type."""
     return t if t.dtype == like.dtype and t.is_contiguous() else t.to(like.dtype).contiguous()
@@ -2165,24 +2174,20 @@ class LayerNorm(torch.autograd.Function):
         C = x.shape[-1] if x.dim() else 0
         if C == 0:
             raise RuntimeError(f'layer norm: the last dimension must hold values, got {tuple(x.shape)}')
-        for p, what in ((weight, 'weight'), (bias, 'bias')):
-            if p is not None:
-                _check_device(p, f'layer norm {what}')
-                if p.dtype != torch.float32 or p.shape != (C,):
-                    raise RuntimeError(f'layer norm {what}: fp32 [{C}], got {p.dtype} {tuple(p.shape)}')
-        code = _dt(x)
+        if weight is not None:
+            weight = _param(weight, x, torch.float32, (C,), 'layer norm weight')
+        if bias is not None:
+            bias = _param(bias, x, torch.float32, (C,), 'layer norm bias')
         x2, rows, ldx = _rows(x, 'layer norm')
-        d = L.NormDesc(rows, C, ldx, eps, code)
-        weight = weight.contiguous() if weight is not None else None
-        bias = bias.contiguous() if bias is not None else None
+        d = L.NormDesc(rows, C, ldx, eps, _dt(x))
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         stats = m = r = None
         if any(ctx.needs_input_grad):
             stats = torch.empty(2 * rows, dtype=torch.float32, device=y.device)      # means, then 1 / deviations
             m = stats.data_ptr()
             r = m + 4 * rows
-        L.check(lib.vfd_layer_norm_fwd(ctypes.byref(d), x2.data_ptr(), L.ptr(weight), L.ptr(bias), y.data_ptr(), m, r,
-                                       L.stream()), 'layer_norm_fwd')
+        L.check(lib.vfd_layer_norm_fwd(d, x2.data_ptr(), L.ptr(weight), L.ptr(bias), y.data_ptr(), m, r, L.stream()),
+                'layer_norm_fwd')
         if L.PROF_ON:
             L.ALG_BYTES['layer_norm_fwd'] += 2 * x.numel() * x.element_size()
         ctx.d = d
@@ -2198,14 +2203,14 @@ class LayerNorm(torch.autograd.Function):
         g = _as(g, x)
         dx = torch.empty_like(g) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
-        db = (torch.empty(d.cols, dtype=torch.float32, device=g.device) if weight is None else torch.empty_like(weight)) if need_b else None
+        db = torch.empty(d.cols, dtype=torch.float32, device=g.device) if need_b else None
         ws, nws = None, 0
         if need_w or need_b:
-            nws = lib.vfd_layer_norm_bwd_workspace(ctypes.byref(d))
-            ws = _ws(nws, x.device)
+            nws = lib.vfd_layer_norm_bwd_workspace(d)
+            ws = _ws(nws, g.device)
         m = stats.data_ptr()
-        L.check(lib.vfd_layer_norm_bwd(ctypes.byref(d), g.data_ptr(), x.data_ptr(), L.ptr(weight), m, m + 4 * d.rows,
-                                       L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), nws, L.stream()), 'layer_norm_bwd')
+        L.check(lib.vfd_layer_norm_bwd(d, g.data_ptr(), x.data_ptr(), L.ptr(weight), m, m + 4 * d.rows, L.ptr(dx), L.ptr(dw),
+                                       L.ptr(db), L.ptr(ws), nws, L.stream()), 'layer_norm_bwd')
         if L.PROF_ON:
             L.ALG_BYTES['layer_norm_bwd'] += (2 + need_x) * g.numel() * g.element_size()
         return dx, dw, db, None
@@ -2231,25 +2236,24 @@ class LinearAct(torch.autograd.Function):
             raise RuntimeError(f'linear: x [..., K] and weight [N, K], K and N at least 1, got {tuple(x.shape)} and '
                                f'{tuple(getattr(weight, "shape", ()))}')
         N, K = weight.shape
+        dtype, shape = x.dtype, (*x.shape[:-1], N)
         code = _dt(x)
-        for t, what, shape in ((weight, 'weight', (N, K)), (bias, 'bias', (N,)),
-                               (residual, 'residual', (*x.shape[:-1], N))):
-            if t is not None:
-                _check_device(t, f'linear {what}')
-                if t.dtype != x.dtype or t.shape != shape:
-                    raise RuntimeError(f'linear {what}: {x.dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}')
+        weight = _param(weight, x, dtype, (N, K), 'linear weight')
+        if bias is not None:
+            bias = _param(bias, x, dtype, (N,), 'linear bias')
+        if residual is not None:
+            residual = _param(residual, x, dtype, shape, 'linear residual')
         x2, rows, ldx = _rows(x, 'linear')
         d = L.LinearDesc(rows, K, N, L.LINEAR_ACTS[act], ldx, code)
-        weight = weight.contiguous()
-        bias = bias.contiguous() if bias is not None else None
-        residual = residual.contiguous() if residual is not None else None
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-        keep = d.act != 0 and any(ctx.needs_input_grad[:3])
-        z = torch.empty(rows, N, dtype=x.dtype, device=x.device) if keep else None
-        nws = lib.vfd_linear_workspace(ctypes.byref(d), L.LINEAR_FWD)
-        ws = _ws(nws, x.device) if nws else None
-        L.check(lib.vfd_linear_fwd(ctypes.byref(d), x2.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(residual),
-                                   y.data_ptr(), L.ptr(z), L.ptr(ws), nws, L.stream()), 'linear_fwd')
+        y = torch.empty(shape, dtype=dtype, device=x.device)
+        z = None
+        if d.act and any(ctx.needs_input_grad[:3]):
+            z = torch.empty_like(y)
+        ws, nws = None, lib.vfd_linear_fwd_workspace(d)
+        if nws:
+            ws = _ws(nws, y.device)
+        L.check(lib.vfd_linear_fwd(d, x2.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(residual), y.data_ptr(), L.ptr(z),
+                                   L.ptr(ws), nws, L.stream()), 'linear_fwd')
         if L.PROF_ON:
             L.ALG_BYTES['linear_fwd'] += x.element_size() * (x.numel() + weight.numel() + y.numel()
                                                              * (1 + (z is not None) + (residual is not None)))
@@ -2262,31 +2266,24 @@ class LinearAct(torch.autograd.Function):
         lib = L.load()
         x, weight, z = ctx.saved_tensors
         d = ctx.d
-        need = ctx.needs_input_grad
-        lead = g.shape[:-1]
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dr = g if need_r else None
+        if not (need_x or need_w or need_b):
+            return None, None, None, dr, None
         g = _as(g, x)
-        new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)  # noqa: E731
-
-        def call(fn, what, *args):
-            nws = lib.vfd_linear_workspace(ctypes.byref(d), what)
-            ws = _ws(nws, x.device) if nws else None
-            L.check(fn(ctypes.byref(d), *args, L.ptr(ws), nws, L.stream()), fn.__name__)
-        db = new(d.n) if need[2] else None
-        gz = g
-        if any(need[:3]) and (d.act != 0 or need[2]):
-            gz = new(d.rows, d.n) if d.act else g
-            call(lib.vfd_linear_act_bwd, L.LINEAR_ACT_BWD, g.data_ptr(), L.ptr(z), gz.data_ptr(), L.ptr(db))
-        dx = dw = None
-        if need[0]:
-            dx = new(*lead, d.k)
-            call(lib.vfd_linear_dgrad, L.LINEAR_DGRAD, gz.data_ptr(), weight.data_ptr(), dx.data_ptr())
-        if need[1]:
-            dw = new(d.n, d.k)
-            call(lib.vfd_linear_wgrad, L.LINEAR_WGRAD, gz.data_ptr(), x.data_ptr(), dw.data_ptr())
+        dx = torch.empty((*g.shape[:-1], d.k), dtype=g.dtype, device=g.device) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty(d.n, dtype=g.dtype, device=g.device) if need_b else None
+        nws = lib.vfd_linear_bwd_workspace(d)
+        at = -(-nws // 256) * 256                       # the gradient behind the activation lies behind the workspace
+        ws = _ws(at + (g.numel() * g.element_size() if d.act else 0), g.device)
+        p = ws.data_ptr()
+        L.check(lib.vfd_linear_bwd(d, g.data_ptr(), L.ptr(z), weight.data_ptr(), x.data_ptr(), p + at, L.ptr(dx), L.ptr(dw),
+                                   L.ptr(db), p, nws, L.stream()), 'linear_bwd')
         if L.PROF_ON:
-            L.ALG_BYTES['linear_bwd'] += x.element_size() * (g.numel() * (1 + 2 * (d.act != 0)) + (need[0] + need[1])
+            L.ALG_BYTES['linear_bwd'] += x.element_size() * (g.numel() * (1 + 2 * (d.act != 0)) + (need_x + need_w)
                                                              * (g.numel() + x.numel() + weight.numel()))
-        return dx, dw, db, (g if need[3] else None), None
+        return dx, dw, db, dr, None
 
 
 # =============================================================================================
