@@ -249,47 +249,47 @@ struct LinEpi {
   int act;
 };
 
-// Eight consecutive values at any element boundary, `cnt` of them (the rest 0); null: 0
-template <typename T>
-__device__ __forceinline__ void lin_ld8(const T* __restrict__ p, int cnt, float (&f)[8]) {
-  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  if (p != nullptr && cnt == 8) {
-    const v8 v = *reinterpret_cast<const v8*>(p);
+// V consecutive values at any element boundary, `cnt` of them (the rest 0); null: 0
+template <int V, typename T>
+__device__ __forceinline__ void lin_ld(const T* __restrict__ p, int cnt, float (&f)[V]) {
+  typedef T vv __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  if (p != nullptr && cnt == V) {
+    const vv v = *reinterpret_cast<const vv*>(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+    for (int e = 0; e < V; ++e) f[e] = (float)v[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (p != nullptr && e < cnt) ? ld1(p + e) : 0.f;
+    for (int e = 0; e < V; ++e) f[e] = (p != nullptr && e < cnt) ? ld1(p + e) : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void lin_st8(T* __restrict__ p, int cnt, const float (&f)[8]) {
-  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  if (cnt == 8) {
-    v8 v;
+template <int V, typename T>
+__device__ __forceinline__ void lin_st(T* __restrict__ p, int cnt, const float (&f)[V]) {
+  typedef T vv __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  if (cnt == V) {
+    vv v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (T)f[e];
-    *reinterpret_cast<v8*>(p) = v;
+    for (int e = 0; e < V; ++e) v[e] = (T)f[e];
+    *reinterpret_cast<vv*>(p) = v;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < V; ++e)
       if (e < cnt) st1(p + e, f[e]);
   }
 }
 
-// The epilogue of eight consecutive outputs at element `at` of y
-template <int ACT, typename T>
-__device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[8], const float (&res)[8],
-                                           float (&v)[8]) {
+// The epilogue of V consecutive outputs at element `at` of y
+template <int ACT, int V, typename T>
+__device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[V], const float (&res)[V],
+                                           float (&v)[V]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += bias[e];
-  if (ep.z) lin_st8(ep.z + at, cnt, v);
+  for (int e = 0; e < V; ++e) v[e] += bias[e];
+  if (ep.z) lin_st<V>(ep.z + at, cnt, v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = lin_act<ACT>(v[e]) + res[e];
-  lin_st8(ep.y + at, cnt, v);
+  for (int e = 0; e < V; ++e) v[e] = lin_act<ACT>(v[e]) + res[e];
+  lin_st<V>(ep.y + at, cnt, v);
 }
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC, int ACT>
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC, bool PART, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinOp<T> w, LinEpi<T> ep, int tm, int tn, int splits) {
   constexpr int NT = 64 * WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
   typedef LinT<T> X;
@@ -427,16 +427,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
   }
 
   // D of a block: column (lane & 31) = row of y, 4 consecutive columns of y per group of 4 registers.  Each wave turns 32
-  // rows at a time over in its own part of LDS, so that its lanes store (and load residuals) 8 consecutive columns each,
-  // whole lines of a row together: stored from registers, 32 bytes of 32 rows at a time, the same outputs took up to
-  // twice as long (92 160 x 1024 bf16, contraction 256: 197 us, 120 this way).  The pitch of 4 more floats spreads the
-  // rows over the banks.
-  constexpr int COLS = FN * 32, PITCH = COLS + 4, LPR = COLS / 8, PASS = 64 / LPR;
+  // rows at a time over in its own part of LDS, so that its lanes store (and load residuals) 16 bytes each, whole lines of
+  // a row together: stored from registers, 32 bytes of 32 rows at a time, the same outputs took up to twice as long
+  // (92 160 x 1024 bf16, contraction 256: 197 us, 120 this way).  The pitch of 4 more floats spreads the rows over the banks.
+  constexpr int COLS = FN * 32, PITCH = COLS + 4;
   static_assert(WM * WN * 32 * PITCH * 4 <= SLOTS * STAGE, "the waves' output rows fit where the tiles were");
   float* turn = reinterpret_cast<float*>(lds) + wave * (32 * PITCH);
-  const int M = x.O, N = w.O, col = n0 + wn + (lane % LPR) * 8, cnt = min(max(N - col, 0), 8);
-  float bias[8];
-  lin_ld8(ep.bias && ep.part == nullptr ? ep.bias + col : nullptr, cnt, bias);
+  const int M = x.O, N = w.O;
   auto turn_over = [&](auto i) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
@@ -448,8 +445,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
         *reinterpret_cast<lin_f4*>(turn + (lane & 31) * PITCH + 32 * j + 8 * q + 4 * (lane >> 5)) = v;
       }
   };
+  constexpr int V = PART ? 4 : X::VE, LPR = COLS / V, PASS = 64 / LPR;
+  const int col = n0 + wn + (lane % LPR) * V, cnt = min(max(N - col, 0), V);
+  float bias[V];
+  if constexpr (!PART) lin_ld<V>(ep.bias ? ep.bias + col : nullptr, cnt, bias);
 #pragma unroll 1
-  for (int i = 0; i < FM; ++i) {                           // one copy of the epilogue's code
+  for (int i = 0; i < FM; ++i) {                         // one copy of the epilogue's code
     if (i == 0) turn_over(std::integral_constant<int, 0>());
     if constexpr (FM > 1)
       if (i == 1) turn_over(std::integral_constant<int, 1>());
@@ -460,8 +461,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 4 * PASS) {            // four rows a lane in flight
-      float v[4][8], res[4][8];
+    for (int r0 = 0; r0 < 32; r0 += 4 * PASS) {          // four rows a lane in flight
+      float v[4][V], res[4][V];
       int c[4];
       size_t at[4];
 #pragma unroll
@@ -469,18 +470,18 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
         const int r = r0 + u * PASS + lane / LPR, m = m0 + wm + 32 * i + r;
         c[u] = m < M ? cnt : 0;
         at[u] = (size_t)m * N + col;
-        lin_ld8(ep.res && ep.part == nullptr ? ep.res + at[u] : nullptr, c[u], res[u]);
+        if constexpr (!PART) lin_ld<V>(ep.res ? ep.res + at[u] : nullptr, c[u], res[u]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const lin_f4 t = *reinterpret_cast<const lin_f4*>(turn + r * PITCH + (lane % LPR) * 8 + 4 * h);
+        for (int h = 0; h < V / 4; ++h) {
+          const lin_f4 t = *reinterpret_cast<const lin_f4*>(turn + r * PITCH + (lane % LPR) * V + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[u][4 * h + e] = t[e];
         }
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (ep.part)
-          lin_st8(ep.part + (size_t)split * M * N + at[u], c[u], v[u]);
+        if constexpr (PART)
+          lin_st<V>(ep.part + (size_t)split * M * N + at[u], c[u], v[u]);
         else
           lin_finish<ACT>(ep, at[u], c[u], bias, res[u], v[u]);
       }
@@ -576,29 +577,26 @@ __global__ __launch_bounds__(512) void lin_thin_k(LinOp<T> x, LinOp<T> w, LinEpi
 // A split contraction's partial products, added in split order, and the epilogue.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int M, int N) {
-  const int rows8 = (N + 7) / 8;                           // eight columns a thread
-  const size_t mn = (size_t)M * N, all = (size_t)M * rows8;
+  constexpr int V = 4, U = 4;                              // columns a thread, partials in flight
+  const int chunks = (N + V - 1) / V;
+  const size_t mn = (size_t)M * N, all = (size_t)M * chunks;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
-    const size_t m = i / rows8;
-    const int col = (int)(i - m * rows8) * 8, cnt = min(N - col, 8);
+    const size_t m = i / chunks;
+    const int col = (int)(i - m * chunks) * V, cnt = min(N - col, V);
     const float* p = ep.part + m * N + col;
-    float v[8], a[8], b[8];
-    lin_ld8(p, cnt, v);
-    int k = 1;
-    for (; k + 1 < splits; k += 2) {
-      lin_ld8(p + k * mn, cnt, a);
-      lin_ld8(p + (k + 1) * mn, cnt, b);
+    float v[V], a[U][V];
+    lin_ld<V>(p, cnt, v);
+    for (int k = 1; k < splits; k += U) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (v[e] + a[e]) + b[e];
-    }
-    if (k < splits) {
-      lin_ld8(p + k * mn, cnt, a);
+      for (int u = 0; u < U; ++u) lin_ld<V>(k + u < splits ? p + (k + u) * mn : nullptr, cnt, a[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += a[e];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += a[u][e];
     }
-    lin_ld8(ep.bias ? ep.bias + col : nullptr, cnt, b);
-    lin_ld8(ep.res ? ep.res + m * N + col : nullptr, cnt, a);
-    lin_finish<ACT>(ep, m * N + col, cnt, b, a, v);
+    lin_ld<V>(ep.bias ? ep.bias + col : nullptr, cnt, a[0]);
+    lin_ld<V>(ep.res ? ep.res + m * N + col : nullptr, cnt, a[1]);
+    lin_finish<ACT>(ep, m * N + col, cnt, a[0], a[1], v);
   }
 }
 
@@ -705,32 +703,33 @@ static LinPlan lin_plan(int M, int N, int K, int resident) {
   return p;
 }
 
-template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC>
+template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC, bool SPLIT>
 static int lin_launch(const LinOp<T>& x, const LinOp<T>& w, LinEpi<T> ep, const LinPlan& p, float* part, hipStream_t s) {
   constexpr int bytes = SLOTS * (BM + BN) * RB;
   ep.part = p.splits > 1 ? part : nullptr;
   const unsigned grid = (unsigned)(p.tm * p.tn * p.splits);
-  auto launch = [&](auto act) {
-    auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN, OCC, RB, SLOTS, ASYNC, act()>;
+  auto launch = [&](auto part_, auto act) {
+    auto* fn = lin_tile_k<T, XMC, WMC, BM, BN, WM, WN, OCC, RB, SLOTS, ASYNC, part_(), act()>;
     lds_attr((const void*)fn, bytes);
     fn<<<grid, 64 * WM * WN, bytes, s>>>(x, w, ep, p.tm, p.tn, p.splits);
     return 0;
   };
-  if constexpr (XMC || WMC) {                              // gradients have no activation of their own
-    launch(std::integral_constant<int, LIN_NONE>());
-  } else {
-    if (p.splits > 1)
-      launch(std::integral_constant<int, LIN_NONE>());
-    else
-      lin_with_act(ep.act, launch);
+  const std::integral_constant<int, LIN_NONE> none;
+  if constexpr (SPLIT) {
+    if (p.splits > 1) {
+      launch(std::true_type(), none);
+      const size_t blocks = ((size_t)x.O * ((w.O + 3) / 4) + 255) / 256;
+      lin_with_act(ep.act, [&](auto act) {
+        lin_join_k<T, act()><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, x.O, w.O);
+        return 0;
+      });
+      return fail_launch("linear");
+    }
   }
-  if (p.splits > 1) {
-    const size_t blocks = ((size_t)x.O * ((w.O + 7) / 8) + 255) / 256;
-    lin_with_act(ep.act, [&](auto act) {
-      lin_join_k<T, act()><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(ep, p.splits, x.O, w.O);
-      return 0;
-    });
-  }
+  if constexpr (XMC || WMC)                                // gradients have no activation of their own
+    launch(std::false_type(), none);
+  else
+    lin_with_act(ep.act, [&](auto act) { return launch(std::false_type(), act); });
   return fail_launch("linear");
 }
 
@@ -792,13 +791,13 @@ static int lin_sized(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, 
   const LinChoice c = lin_choose<T, XMC, WMC>(x.O, w.O, x.K, ASYNC);
   if constexpr (ASYNC) {
     if constexpr (sizeof(T) == 2)
-      if (c.form == LIN_F_BIG) return lin_launch<T, XMC, WMC, 256, 256, 2, 4, 2, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
+      if (c.form == LIN_F_BIG) return lin_launch<T, XMC, WMC, 256, 256, 2, 4, 2, 128, 2, ASYNC, false>(x, w, ep, c.plan, part, s);
     if constexpr (sizeof(T) == 4)
-      if (c.form == LIN_F_FLAT) return lin_launch<T, XMC, WMC, 64, 128, 2, 2, 3, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
+      if (c.form == LIN_F_FLAT) return lin_launch<T, XMC, WMC, 64, 128, 2, 2, 3, 128, 2, ASYNC, false>(x, w, ep, c.plan, part, s);
   }
   if constexpr (!XMC)
-    if (c.form == LIN_F_SHORT) return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 3, 64, 3, ASYNC>(x, w, ep, c.plan, part, s);
-  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, 128, 2, ASYNC>(x, w, ep, c.plan, part, s);
+    if (c.form == LIN_F_SHORT) return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 3, 64, 3, ASYNC, true>(x, w, ep, c.plan, part, s);
+  return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, 128, 2, ASYNC, true>(x, w, ep, c.plan, part, s);
 }
 
 template <typename T, bool XMC, bool WMC>
