@@ -249,11 +249,15 @@ struct LinEpi {
   int act;
 };
 
-// V consecutive values at any element boundary, `cnt` of them (the rest 0); null: 0
+// V consecutive values at any element boundary, `cnt` of them (the rest 0); null: 0; whole: all of them in every lane
 template <int V, typename T>
-__device__ __forceinline__ void lin_ld(const T* __restrict__ p, int cnt, float (&f)[V]) {
+__device__ __forceinline__ void lin_ld(const T* __restrict__ p, int cnt, float (&f)[V], bool whole = false) {
   typedef T vv __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-  if (p != nullptr && cnt == V) {
+  if (whole) {
+    const vv v = *reinterpret_cast<const vv*>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = (float)v[e];
+  } else if (p != nullptr && cnt == V) {
     const vv v = *reinterpret_cast<const vv*>(p);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = (float)v[e];
@@ -263,30 +267,36 @@ __device__ __forceinline__ void lin_ld(const T* __restrict__ p, int cnt, float (
   }
 }
 template <int V, typename T>
-__device__ __forceinline__ void lin_st(T* __restrict__ p, int cnt, const float (&f)[V]) {
+__device__ __forceinline__ void lin_st(T* __restrict__ p, int cnt, const float (&f)[V], bool whole = false) {
   typedef T vv __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-  if (cnt == V) {
-    vv v;
+  vv v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (T)f[e];
+  for (int e = 0; e < V; ++e) v[e] = (T)f[e];
+  if (whole) {
+    *reinterpret_cast<vv*>(p) = v;
+  } else if (cnt == V) {
     *reinterpret_cast<vv*>(p) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (e < cnt) st1(p + e, f[e]);
+      if (e < cnt) p[e] = v[e];
   }
 }
 
 // The epilogue of V consecutive outputs at element `at` of y
 template <int ACT, int V, typename T>
 __device__ __forceinline__ void lin_finish(const LinEpi<T>& ep, size_t at, int cnt, const float (&bias)[V], const float (&res)[V],
-                                           float (&v)[V]) {
+                                           float (&v)[V], bool whole = false) {
+  if (ep.bias)
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] += bias[e];
-  if (ep.z) lin_st<V>(ep.z + at, cnt, v);
+    for (int e = 0; e < V; ++e) v[e] += bias[e];
+  if (ep.z) lin_st<V>(ep.z + at, cnt, v, whole);
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = lin_act<ACT>(v[e]) + res[e];
-  lin_st<V>(ep.y + at, cnt, v);
+  for (int e = 0; e < V; ++e) v[e] = lin_act<ACT>(v[e]);
+  if (ep.res)
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += res[e];
+  lin_st<V>(ep.y + at, cnt, v, whole);
 }
 
 template <typename T, bool XMC, bool WMC, int BM, int BN, int WM, int WN, int OCC, int RB, int SLOTS, bool ASYNC, bool PART, int ACT>
@@ -447,8 +457,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
   };
   constexpr int V = PART ? 4 : X::VE, LPR = COLS / V, PASS = 64 / LPR;
   const int col = n0 + wn + (lane % LPR) * V, cnt = min(max(N - col, 0), V);
+  const bool whole = m0 + BM <= M && n0 + BN <= N;       // no edge in this tile (uniform)
   float bias[V];
-  if constexpr (!PART) lin_ld<V>(ep.bias ? ep.bias + col : nullptr, cnt, bias);
+  if constexpr (!PART)
+    if (ep.bias) lin_ld<V>(ep.bias + col, cnt, bias, whole);
+  size_t row = (size_t)(m0 + wm + lane / LPR) * N + col;
+  const size_t down = (size_t)PASS * N;
 #pragma unroll 1
   for (int i = 0; i < FM; ++i) {                         // one copy of the epilogue's code
     if (i == 0) turn_over(std::integral_constant<int, 0>());
@@ -464,13 +478,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
     for (int r0 = 0; r0 < 32; r0 += 4 * PASS) {          // four rows a lane in flight
       float v[4][V], res[4][V];
       int c[4];
-      size_t at[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int r = r0 + u * PASS + lane / LPR, m = m0 + wm + 32 * i + r;
-        c[u] = m < M ? cnt : 0;
-        at[u] = (size_t)m * N + col;
-        if constexpr (!PART) lin_ld<V>(ep.res ? ep.res + at[u] : nullptr, c[u], res[u]);
+        const int r = r0 + u * PASS + lane / LPR;
+        c[u] = m0 + wm + 32 * i + r < M ? cnt : 0;
+        if constexpr (!PART)
+          if (ep.res) lin_ld<V>(ep.res + row + u * down, c[u], res[u], whole);
 #pragma unroll
         for (int h = 0; h < V / 4; ++h) {
           const lin_f4 t = *reinterpret_cast<const lin_f4*>(turn + r * PITCH + (lane % LPR) * V + 4 * h);
@@ -481,10 +494,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if constexpr (PART)
-          lin_st<V>(ep.part + (size_t)split * M * N + at[u], c[u], v[u]);
+          lin_st<V>(ep.part + (size_t)split * M * N + row + u * down, c[u], v[u], whole);
         else
-          lin_finish<ACT>(ep, at[u], c[u], bias, res[u], v[u]);
+          lin_finish<ACT>(ep, row + u * down, c[u], bias, res[u], v[u], whole);
       }
+      row += 4 * down;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
