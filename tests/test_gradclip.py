@@ -286,6 +286,21 @@ def test_parameters_and_a_parameter_listed_twice():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """One tensor of 2.2 billion values, all zero but for a few at its ends."""
+    from vfdepth_amd import kernels as KN
+    g = torch.zeros((1 << 31) + 70001, dtype=BF16, device='cuda')
+    g[:3], g[-5:] = 3.0, 4.0
+    n = math.sqrt(3 * 9 + 5 * 16)
+    out = torch.full(g.shape, 7.0, dtype=BF16, device='cuda')
+    got = KN.clip_grads([g], 1.0, out=[out])
+    assert abs(float(got) - n) <= HALF[F32] * n * (1 + 1e-6)
+    _near(out[:3], g[:3].cpu().double() / (n + 1e-6), (HALF[F32] + HALF[BF16]) * (1 + 1e-6))
+    _near(out[-5:], g[-5:].cpu().double() / (n + 1e-6), (HALF[F32] + HALF[BF16]) * (1 + 1e-6))
+    assert int(out.count_nonzero()) == 8
+
+
+@gpu
 def test_another_stream_and_a_captured_graph():
     from vfdepth_amd import kernels as KN
     src = _make([5000, 17, 123], F32)

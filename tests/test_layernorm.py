@@ -287,6 +287,23 @@ def test_module_parameters_in_bf16_and_autocast():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """2.2 billion values: the last rows are the same as on their own, and nothing wraps onto the first ones."""
+    from vfdepth_amd import kernels as KN
+    rows, C = (1 << 21) + 5, 1024
+    x = torch.empty(rows, C, dtype=BF16, device='cuda').normal_()
+    g = torch.empty(rows, C, dtype=BF16, device='cuda').normal_()
+    w, b = torch.randn(C, device='cuda'), torch.randn(C, device='cuda')
+    y = KN.LayerNorm.apply(x.requires_grad_(True), w, b, EPS)
+    dx, = torch.autograd.grad(y, x, g)
+    for part in (slice(0, 7), slice(rows - 9, rows)):
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys = KN.LayerNorm.apply(xs, w, b, EPS)
+        ds, = torch.autograd.grad(ys, xs, g[part].clone())
+        assert torch.equal(y[part], ys) and torch.equal(dx[part], ds)
+
+
+@gpu
 def test_streams_and_captured_graph():
     from vfdepth_amd import kernels as KN
     x, w, b, g = (t.cuda() for t in _case(500, 200, F32, seed=9))

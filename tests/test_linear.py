@@ -358,6 +358,30 @@ def test_autocast():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """Input, output and weight-gradient reads of 2.2 billion values each: rows at both ends against the oracle."""
+    from vfdepth_amd import kernels as KN
+    M, K, N = (1 << 21) + 37, 1032, 1032
+    x = torch.empty(M, K, dtype=BF16, device='cuda').normal_()
+    w = (torch.randn(N, K, device='cuda') * K ** -0.5).to(BF16)
+    b = torch.randn(N, device='cuda').to(BF16)
+    with torch.no_grad():
+        y = KN.LinearAct.apply(x, w, b, None, 'gelu')
+    for part in (slice(0, 40), slice(M - 300, M)):
+        vals, tol = _oracle(x[part], w, b, None, torch.zeros(1, N), 'gelu')
+        _check([y[part]], vals, tol)
+    # the weight's gradient of rows that are zero but for the last ones: theirs alone
+    g = torch.zeros(M, N, dtype=BF16, device='cuda')
+    g[-20:] = torch.randn(20, N, device='cuda').to(BF16)
+    wg = w.clone().requires_grad_(True)
+    xg = x.requires_grad_(True)
+    dx, dw = torch.autograd.grad(KN.LinearAct.apply(xg, wg, b, None, 'none'), (xg, wg), g)
+    vals, tol = _oracle(x[-20:], w, b, None, g[-20:], 'none')
+    _check([None, dx[-20:], dw], vals, tol)
+    assert not dx[:1000].any()
+
+
+@gpu
 @pytest.mark.parametrize('dtype', [F32, BF16])
 def test_streams_and_captured_graph(dtype):
     from vfdepth_amd import kernels as KN

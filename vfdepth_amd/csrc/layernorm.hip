@@ -347,7 +347,7 @@ constexpr int LN_FWD_GRID = 2048;
 
 // Blocks of the backward = partial rows: enough to keep every CU loading, few enough that the partials (8 C bytes each,
 // written and read) stay small beside the rows.
-static int ln_bwd_blocks(int rows, int C, int rb, int w) {
+static int ln_bwd_blocks(int rows, int rb, int w) {
   const int most = w > 1 ? 512 : 1024;
   const int need = (rows + rb - 1) / rb;
   return need < most ? need : most;
@@ -359,7 +359,7 @@ static int ln_parts(int rows, int C) {
     if constexpr (decltype(l)::value == 0)
       return rows < 128 ? rows : 128;
     else
-      return ln_bwd_blocks(rows, C, LnGroup<T, l(), w(), nv()>::RB, w());
+      return ln_bwd_blocks(rows, LnGroup<T, l(), w(), nv()>::RB, w());
   });
 }
 

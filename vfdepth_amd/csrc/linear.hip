@@ -29,9 +29,10 @@ __device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2
 // t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), within 1.5e-7 for x >= 0.
 __device__ __forceinline__ float lin_phi(float z, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-  e = lin_exp(-0.5f * z * z);
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float q = 0.5f * p * e;
+  e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504088896341f));
+  const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f),
+                       0.5f * 0.254829592f);
+  const float q = t * p * e;
   return z > 0.f ? 1.f - q : q;
 }
 
@@ -463,6 +464,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
     if (ep.bias) lin_ld<V>(ep.bias + col, cnt, bias, whole);
   size_t row = (size_t)(m0 + wm + lane / LPR) * N + col;
   const size_t down = (size_t)PASS * N;
+  constexpr int FLY = OCC > 2 ? 2 : 4;                     // (three blocks a CU leave fewer registers)
 #pragma unroll 1
   for (int i = 0; i < FM; ++i) {                         // one copy of the epilogue's code
     if (i == 0) turn_over(std::integral_constant<int, 0>());
@@ -475,11 +477,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 4 * PASS) {          // four rows a lane in flight
-      float v[4][V], res[4][V];
-      int c[4];
+    for (int r0 = 0; r0 < 32; r0 += FLY * PASS) {        // rows a lane in flight
+      float v[FLY][V], res[FLY][V];
+      int c[FLY];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < FLY; ++u) {
         const int r = r0 + u * PASS + lane / LPR;
         c[u] = m0 + wm + 32 * i + r < M ? cnt : 0;
         if constexpr (!PART)
@@ -492,13 +494,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < FLY; ++u) {
         if constexpr (PART)
           lin_st<V>(ep.part + (size_t)split * M * N + row + u * down, c[u], v[u], whole);
         else
           lin_finish<ACT>(ep, row + u * down, c[u], bias, res[u], v[u], whole);
       }
-      row += 4 * down;
+      row += FLY * down;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
