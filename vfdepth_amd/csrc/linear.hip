@@ -721,18 +721,35 @@ struct LinPlan {
   int tm, tn, splits;
 };
 
-// Tiles of BM x BN, and how often the contraction is split so that a product with few tiles still fills the chip (a
-// split keeps at least four staged tiles of work).
-template <typename T, int BM, int BN>
-static LinPlan lin_plan(int M, int N, int K, int resident) {
-  constexpr int BK = 128 / (int)sizeof(T);
-  LinPlan p;
-  p.tm = (M + BM - 1) / BM;
-  p.tn = (N + BN - 1) / BN;
+// How often the contraction of a product of 128 x 128 tiles is split: the cheapest of splits that fill one, two or three
+// blocks a CU, of a few small ones and of none.  A block's 128 bytes of contraction take `lat` microseconds where it is
+// alone on its CU and `thr` of the CU's time where it is not (both measured: fp32, bound by the matrix cores, 1.9 and 1.8;
+// bf16 0.55 and 0.47, 0.15 and 0.03 more for each operand that is read across; staged through registers 0.85 more, and 0.6
+// for each read across); a round starts and stores in 3, a second launch takes 6 and the partial sums their bytes at 8 TB/s
+// (from cache).  1472 x 512 x 768 bf16: 8.9 us unsplit, 13.3 in two; 2000 x 512 x 512 fp32: 24 in four, 27 in two.
+template <typename T, bool XMC, bool WMC>
+static LinPlan lin_plan(int M, int N, int K, int resident, bool aligned) {
+  constexpr int BK = 128 / (int)sizeof(T), ACROSS = (int)XMC + (int)WMC;
+  const double lat = (sizeof(T) == 4 ? 1.9 : 0.55 + 0.15 * ACROSS) + (aligned ? 0.0 : 0.85 + 0.6 * ACROSS);
+  const double thr = sizeof(T) == 4 ? 1.8 : 0.47 + 0.03 * ACROSS;
+  LinPlan p{(M + 127) / 128, (N + 127) / 128, 1};
   const long long tiles = (long long)p.tm * p.tn, kt = (K + BK - 1) / BK;
-  long long s = (long long)LIN_CUS * resident / tiles;
-  if (s > kt / 4) s = kt / 4;
-  p.splits = s < 1 ? 1 : (int)s;
+  auto cost = [&](long long s) {
+    const long long a_cu = (tiles * s + LIN_CUS - 1) / LIN_CUS, rounds = (a_cu + resident - 1) / resident;
+    const double step = std::max(lat * (double)rounds, thr * (double)a_cu);
+    return (double)((kt + s - 1) / s) * step + 3.0 * (double)rounds + (s > 1 ? 6.0 + (double)s * M * N * 8 / 8e6 : 0.0);
+  };
+  double best = cost(1);
+  auto offer = [&](long long s) {
+    if (s < 2 || s > kt || tiles * s > (long long)LIN_CUS * resident) return;
+    const double c = cost(s);
+    if (c < best) {
+      best = c;
+      p.splits = (int)s;
+    }
+  };
+  for (int c = 1; c <= resident; ++c) offer(LIN_CUS * c / tiles);
+  for (int s = 2; s <= 8; ++s) offer(s);
   return p;
 }
 
@@ -821,8 +838,8 @@ template <typename T, bool XMC, bool WMC>
 static LinChoice lin_choose(int M, int N, int K, bool aligned) {
   if (aligned && lin_big<T>(M, N, K)) return {LIN_F_BIG, LinPlan{(M + 255) / 256, (N + 255) / 256, 1}};
   if (aligned && lin_flat<T>(M, N)) return {LIN_F_FLAT, LinPlan{(M + 63) / 64, (N + 127) / 128, 1}};
-  if (lin_short<XMC>(K)) return {LIN_F_SHORT, lin_plan<T, 128, 128>(M, N, K, 3)};
-  return {LIN_F_LONG, lin_plan<T, 128, 128>(M, N, K, 2)};
+  if (lin_short<XMC>(K)) return {LIN_F_SHORT, lin_plan<T, XMC, WMC>(M, N, K, 3, aligned)};
+  return {LIN_F_LONG, lin_plan<T, XMC, WMC>(M, N, K, 2, aligned)};
 }
 
 template <typename T, bool XMC, bool WMC, bool ASYNC>
