@@ -609,11 +609,12 @@ typedef struct vfd_linear_desc {
 size_t vfd_linear_fwd_workspace(const vfd_linear_desc* d);
 int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z,
                    void* workspace, size_t ws_bytes, void* stream);
-/* From g [rows, n]: gz = g act'(z) (act 0: gz is g, z and gz are not used), dx [rows, k] = gz w, dw [n, k] = gz^T x and
- * db [n] = gz's column sums; dx, dw, db null = not computed.  Fixed-order sums. */
-size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d);
-int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
-                   void* dw, void* db, void* workspace, size_t ws_bytes, void* stream);
+/* From g [rows, n] with gz = g act'(z) (act 0: gz is g, z is not used): dx [rows, k] = gz w, dw [n, k] = gz^T x and db [n] =
+ * gz's column sums; dx, dw, db null = not computed.  Fixed-order sums.  The workspace (which holds gz, and copies of bf16
+ * operands whose pitch or start is odd) depends on the tensors' addresses and on which of dx, dw are asked for. */
+size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d, const void* g, const void* w, const void* x, int dx, int dw);
+int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* dx, void* dw,
+                   void* db, void* workspace, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------ gradient norm / clipping */
 /* Global norm of n gradient tensors (grads[i]: device pointer of numel[i] densely stored elements at any element

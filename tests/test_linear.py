@@ -105,9 +105,9 @@ def test_c_refuses_bad_descriptors(bad):
     d = _desc(**bad)
     p = 1 << 40
     for rc in (lib.vfd_linear_fwd(ctypes.byref(d), p, p, p, p, p, p, p, 1 << 40, None),
-               lib.vfd_linear_bwd(ctypes.byref(d), p, p, p, p, p, p, p, p, p, 1 << 40, None)):
+               lib.vfd_linear_bwd(ctypes.byref(d), p, p, p, p, p, p, p, p, 1 << 40, None)):
         assert rc == -1 and (b'descriptor' in lib.vfd_last_error() or b'tiles' in lib.vfd_last_error())
-    assert lib.vfd_linear_fwd_workspace(ctypes.byref(d)) == lib.vfd_linear_bwd_workspace(ctypes.byref(d)) == 0
+    assert lib.vfd_linear_fwd_workspace(ctypes.byref(d)) == lib.vfd_linear_bwd_workspace(ctypes.byref(d), p, p, p, 1, 1) == 0
 
 
 def test_c_refuses_null_tensors_and_small_workspaces():
@@ -116,17 +116,24 @@ def test_c_refuses_null_tensors_and_small_workspaces():
     p, no = 1 << 40, None
     d = _desc()
 
-    def bwd(g=p, z=no, w=p, x=p, gz=no, dx=p, dw=p, db=p, ws=p, n=1 << 40):
-        return lib.vfd_linear_bwd(ctypes.byref(d), g, z, w, x, gz, dx, dw, db, ws, n, no)
+    def bwd(g=p, z=no, w=p, x=p, dx=p, dw=p, db=p, ws=p, n=1 << 40):
+        return lib.vfd_linear_bwd(ctypes.byref(d), g, z, w, x, dx, dw, db, ws, n, no)
     assert lib.vfd_linear_fwd(ctypes.byref(d), no, p, no, no, p, no, p, 1 << 40, no) == -1
     assert lib.vfd_linear_fwd(ctypes.byref(d), p, p, no, no, no, no, p, 1 << 40, no) == -1
     assert bwd(g=no) == bwd(w=no) == bwd(x=no) == bwd(ws=no) == -1
     assert bwd(dx=no, dw=no, db=no) == 0                                         # nothing asked for: nothing is launched
     d = _desc(act=4)
-    assert bwd(gz=p) == bwd(z=p) == -1 and b'null' in lib.vfd_last_error()
+    assert bwd() == -1 and b'null' in lib.vfd_last_error()
     d = _desc(rows=100000, k=128, n=128, ldx=128)
-    need = lib.vfd_linear_bwd_workspace(ctypes.byref(d))
+    need = lib.vfd_linear_bwd_workspace(ctypes.byref(d), p, p, p, 1, 1)
     assert need > 0 and bwd(n=need - 1) == -1 and b'workspace' in lib.vfd_last_error()
+    assert lib.vfd_linear_bwd_workspace(ctypes.byref(d), p, p, p, 0, 0) < need
+    odd = _desc(rows=50000, k=333, n=77, ldx=333, dtype=1)                       # rows of an odd length are laid out anew
+    even = _desc(rows=50000, k=334, n=78, ldx=334, dtype=1)
+    copies = 2 * (50000 * 80 + 77 * 336 + 50000 * 336)
+    ws = [lib.vfd_linear_bwd_workspace(ctypes.byref(t), p, p, p, 1, 1) for t in (odd, even)]
+    assert ws[0] >= copies and ws[1] < copies
+    assert lib.vfd_linear_bwd_workspace(ctypes.byref(even), p, p, p + 2, 1, 1) >= ws[1] + 2 * 50000 * 336     # an odd start
     d = _desc(rows=300, k=8192, n=128, ldx=8192)                                 # few tiles: the contraction is split
     need = lib.vfd_linear_fwd_workspace(ctypes.byref(d))
     assert need > 0 and lib.vfd_linear_fwd(ctypes.byref(d), p, p, no, no, p, no, p, need - 1, no) == -1
@@ -180,7 +187,8 @@ def test_layer_refusals():
 gpu = pytest.mark.gpu
 SHAPES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (5, 3, 7), (17, 64, 64), (6, 2048, 256), (33, 100, 31), (64, 96, 300), (65, 40, 513),
           (128, 128, 128), (129, 127, 130), (256, 64, 256), (257, 1024, 96), (300, 517, 771), (1000, 8, 2000), (3000, 40, 24),
-          (520, 260, 260), (16, 4096, 512), (9000, 72, 136)]
+          (520, 260, 260), (16, 4096, 512), (9000, 72, 136),
+          (3001, 127, 131), (2100, 259, 130), (700, 1001, 515), (1024, 126, 250), (1500, 131, 258)]
 
 
 @gpu
@@ -209,9 +217,14 @@ def test_activations(act, bias, residual, dtype):
 @gpu
 @pytest.mark.parametrize('dtype', [F32, BF16])
 def test_large_product(dtype):
-    """Enough tiles for the largest tile form, ragged in each direction."""
-    args = _case(4200, 328, 4104, dtype, seed=7)
-    _check(_run(*args, 'silu'), *_oracle(*args, 'silu'))
+    """Enough tiles for the largest tile form, ragged in each direction; odd pitches, whose rows the backward lays out anew."""
+    for M, K, N in ((4200, 1160, 4104), (4100, 333, 771), (4099, 1001, 515)):
+        args = _case(M, K, N, dtype, seed=7)
+        _check(_run(*args, 'silu'), *_oracle(*args, 'silu'))
+        x, w, b, _, g = args
+        args = [x[:, 1:], w[:, 1:].detach(), b, None, g]                # an odd start and a pitch of its own
+        args = [t if t is None else t.detach() for t in args]
+        _check(_run(*args, 'none'), *_oracle(*args, 'none'))
 
 
 @gpu

@@ -175,8 +175,8 @@ _SIGS = {
     'vfd_layer_norm_bwd': (c_int, [ctypes.POINTER(NormDesc)] + [c_fp] * 9 + [c_size_t, c_void_p]),
     'vfd_linear_fwd_workspace': (c_size_t, [ctypes.POINTER(LinearDesc)]),
     'vfd_linear_fwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 7 + [c_size_t, c_void_p]),
-    'vfd_linear_bwd_workspace': (c_size_t, [ctypes.POINTER(LinearDesc)]),
-    'vfd_linear_bwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 9 + [c_size_t, c_void_p]),
+    'vfd_linear_bwd_workspace': (c_size_t, [ctypes.POINTER(LinearDesc)] + [c_fp] * 3 + [c_int] * 2),
+    'vfd_linear_bwd': (c_int, [ctypes.POINTER(LinearDesc)] + [c_fp] * 8 + [c_size_t, c_void_p]),
     'vfd_grad_norm_workspace': (c_size_t, [c_int, c_fp]),
     'vfd_grad_norm': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_fp, c_fp, c_size_t, c_void_p]),
     'vfd_clip_grads': (c_int, [c_int] + [c_fp] * 3 + [c_int, c_double] + [c_fp] * 4 + [c_size_t, c_void_p]),

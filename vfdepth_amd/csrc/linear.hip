@@ -177,7 +177,8 @@ struct LinTile {
     }
   }
   // Whole tiles straight into LDS: a wave's 64 chunks land one after another, so each lane fetches the chunk whose place
-  // that is.  Outer indices beyond the operand fetch its last chunk again (their products are not stored).  Through a
+  // that is.  Outer indices beyond the operand fetch its last chunk again (their products are not stored); a last chunk that
+  // leaves its row goes on into the next one, which a ragged tile of the last rows must not (lin_tile_k).  Through a
   // buffer descriptor: a lane's offsets stay the same for every tile, and past the last tile an empty one loads nothing.
   struct Stream {
     const char* p;                                      // of the next tile (uniform)
@@ -192,7 +193,7 @@ struct LinTile {
     for (int i = 0; i < NCH; ++i) {
       const int e = (int)threadIdx.x + i * NT;
       const int row = e / CPR, c = ((e % CPR) ^ turn(row)) * X::VE;
-      s.off[i] = MC ? (unsigned)row * (unsigned)op.ld * ES + (unsigned)min(c, op.O - X::VE - o0) * ES
+      s.off[i] = MC ? (unsigned)row * (unsigned)op.ld * ES + (unsigned)min(c, (op.O - 1 - o0) / X::VE * X::VE) * ES
                     : (unsigned)min(row, op.O - 1 - o0) * (unsigned)op.ld * ES + c * ES;
     }
   }
@@ -380,7 +381,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
     // SLOTS tiles in LDS: one is worked on, the others are on their way.  The fragments of a step are read during the
     // products of the step before; a tile's last products run behind the barrier that frees its slot, while the next
     // tile's first fragments are read and another tile starts on its way.
-    const int k_end = min(k_hi, x.K / BK);
+    int k_end = min(k_hi, x.K / BK);
+    if (k_end * BK == x.K && ((XMC && x.O % X::VE != 0 && m0 + BM > x.O) || (WMC && w.O % X::VE != 0 && n0 + BN > w.O)))
+      --k_end;                                             // the last row of memory: no row behind it to go on into
     if (k_lo < k_end) {
       typename TX::Stream sx;
       typename TW::Stream sw;
@@ -408,7 +411,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
       }
       lin_arrived<0>();
     }
-    k_lo = max(k_lo, k_end);                             // a last tile that the contraction ends in: staged with masks
+    k_lo = max(k_lo, min(k_end, k_hi));                  // a last tile that the contraction ends in: staged with masks
   }
   {
     typename X::vec vx[TX::NCH], vw[TW::NCH];
@@ -634,11 +637,13 @@ __global__ __launch_bounds__(256) void lin_join_k(LinEpi<T> ep, int splits, int 
 }
 
 // ---------------------------------------------------------------- gz = g act'(z) and its column sums
-// A block owns `cols` = 64 V columns of a strip of rows, four rows at a time (one per wave): gz written as it is read,
-// the columns' sums kept in registers and left as one partial row per block (added in block order by col_sums_k).
+// A block owns 64 V columns of a strip of rows, four rows at a time (one per wave): gz written as it is read, the columns'
+// sums kept in registers and left as one partial row per block (added in block order by col_sums_k).  gz has a pitch of
+// its own, so that rows of an odd length become ones that the products can stream.
+// Measured (16 384 x 8192 bf16, GELU): 185 us, 4.4 TB/s of the 805 MB it reads and writes; 177 without the slope.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, const T* __restrict__ z, T* __restrict__ gz,
-                                                     float* __restrict__ part, int M, int N) {
+                                                     long long ldg, float* __restrict__ part, int M, int N) {
   constexpr int V = LinT<T>::VE;
   typedef typename LinT<T>::vec vec;
   __shared__ float sm[4][64][V + 1];
@@ -691,8 +696,8 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
           s[j] += f[u][j];
           o[j] = (T)f[u][j];
         }
-        if (ACT == LIN_NONE) continue;
-        const size_t at = (size_t)(m0 + u * step) * N + n;
+        if (ACT == LIN_NONE && gz == nullptr) continue;
+        const size_t at = (size_t)(m0 + u * step) * ldg + n;
         if (cnt == V) {
           *reinterpret_cast<vec*>(gz + at) = o;
         } else {
@@ -712,6 +717,22 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
     for (int j = 0; j < V; ++j)
       if (j < cnt)
         part[(size_t)blockIdx.y * N + n + j] = (sm[0][lane][j] + sm[1][lane][j]) + (sm[2][lane][j] + sm[3][lane][j]);
+}
+
+// Rows of an odd pitch or start laid out at a pitch of 16 bytes: read across (the gradients' products), 2-byte rows take 2.5
+// times as long through registers (12 345 x 1001 x 1367 bf16, data and weight gradient 263 us, 131 with this).
+template <typename T>
+__global__ __launch_bounds__(256) void lin_pack_k(const T* __restrict__ src, long long lds, T* __restrict__ dst, long long ldd,
+                                                  int rows, int cols) {
+  const int chunks = (cols + 7) / 8;
+  const size_t all = (size_t)rows * chunks;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / chunks;
+    const int c = (int)(i - r * chunks) * 8;
+    float f[8];
+    lin_ld<8>(src + r * lds + c, min(cols - c, 8), f);
+    lin_st<8>(dst + r * ldd + c, min(cols - c, 8), f);
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -789,12 +810,15 @@ static int lin_launch(const LinOp<T>& x, const LinOp<T>& w, LinEpi<T> ep, const 
   return fail_launch("linear");
 }
 
-// Chunks of 16 bytes at 16-byte boundaries everywhere, and a tile's rows within 31 bits of bytes: what the loads that go
-// straight into LDS take.
+// What the loads that go straight into LDS take: chunks at 4-byte boundaries (all of fp32; bf16 of an even pitch and start)
+// and a tile's rows within 31 bits of bytes.  An operand that is read across fills a chunk in every row.
+template <typename T>
+static bool lin_dwords(const T* p, long long ld) {
+  return (((uintptr_t)p | (uintptr_t)ld * sizeof(T)) & 3) == 0;
+}
 template <typename T, bool MC>
 static bool lin_aligned(const LinOp<T>& op) {
-  constexpr int VE = LinT<T>::VE;
-  return ((uintptr_t)op.p & 15) == 0 && op.ld % VE == 0 && (!MC || op.O % VE == 0) && op.ld < (1 << 20);
+  return lin_dwords(op.p, op.ld) && (!MC || op.O >= LinT<T>::VE) && op.ld < (1 << 20);
 }
 
 // Which tiles a bf16 product takes.  Both measured with their contraction's length (one box, microseconds): a round of 256
@@ -882,12 +906,36 @@ static size_t lin_fwd_ws(const vfd_linear_desc* d) {
   return lin_is_thin(d) ? 0 : lin_part_bytes<T, false, false>(d->rows, d->n, d->k);
 }
 
-// The backward's steps follow each other on one stream through one workspace
+// The backward's workspace: gz (where an activation makes one, or g cannot be streamed), copies of W and x where those
+// cannot, and one scratch for the steps' partial sums, which follow each other on one stream.
+struct LinBwdPlan {
+  long long ldg, ldw, ldx;       // pitches of the operands that the products read
+  bool gz, w, x;                 // whether each is a copy in the workspace
+  size_t at_gz, at_w, at_x, at_part, bytes;
+};
 template <typename T>
-static size_t lin_bwd_ws(const vfd_linear_desc* d) {
+static LinBwdPlan lin_bwd_plan(const vfd_linear_desc* d, const void* g, const void* w, const void* x, bool dx, bool dw) {
+  auto pitch = [](long long n) { return (n + 7) / 8 * 8; };
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  LinBwdPlan p;
+  // a product of few terms is not worth copies of its operands (1471 x 517 x 771: 47 us with and without)
+  const bool pack = (dx || dw) && (double)d->rows * d->k * d->n > 1e9;
+  const bool bad_g = pack && !lin_dwords((const T*)g, d->n);
+  p.gz = d->act != LIN_NONE || bad_g;
+  p.w = pack && dx && !lin_dwords((const T*)w, d->k);
+  p.x = pack && dw && !lin_dwords((const T*)x, d->ldx);
+  p.ldg = p.gz ? pitch(d->n) : d->n;
+  p.ldw = p.w ? pitch(d->k) : d->k;
+  p.ldx = p.x ? pitch(d->k) : d->ldx;
+  p.at_gz = 0;
+  p.at_w = p.at_gz + up(p.gz ? (size_t)d->rows * p.ldg * sizeof(T) : 0);
+  p.at_x = p.at_w + up(p.w ? (size_t)d->n * p.ldw * sizeof(T) : 0);
+  p.at_part = p.at_x + up(p.x ? (size_t)d->rows * p.ldx * sizeof(T) : 0);
   const size_t act = (size_t)lin_strips(d->rows, d->n, LinT<T>::VE) * d->n * sizeof(float);
-  const size_t dx = lin_part_bytes<T, false, true>(d->rows, d->k, d->n), dw = lin_part_bytes<T, true, true>(d->n, d->k, d->rows);
-  return std::max(act, std::max(dx, dw));
+  const size_t sx = dx ? lin_part_bytes<T, false, true>(d->rows, d->k, d->n) : 0;
+  const size_t sw = dw ? lin_part_bytes<T, true, true>(d->n, d->k, d->rows) : 0;
+  p.bytes = p.at_part + std::max(act, std::max(sx, sw));
+  return p;
 }
 
 static int lin_check(const char* what, const vfd_linear_desc* d) {
@@ -920,40 +968,52 @@ static int lin_fwd_run(const vfd_linear_desc* d, const void* x, const void* w, c
 }
 
 template <typename T>
-static int lin_dgrad_run(const vfd_linear_desc* d, const void* gz, const void* w, void* dx, float* part, hipStream_t s) {
-  const LinOp<T> og{(const T*)gz, d->n, d->rows, d->n}, ow{(const T*)w, d->k, d->k, d->n};
-  const LinEpi<T> ep{nullptr, nullptr, nullptr, (T*)dx, nullptr, LIN_NONE};
-  return lin_product<T, false, true>(og, ow, ep, part, s);
+static void lin_pack(const T* src, long long lds, T* dst, long long ldd, int rows, int cols, hipStream_t s) {
+  const size_t chunks = (size_t)rows * ((cols + 7) / 8), blocks = (chunks + 255) / 256;
+  lin_pack_k<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(src, lds, dst, ldd, rows, cols);
 }
 
 template <typename T>
-static int lin_wgrad_run(const vfd_linear_desc* d, const void* gz, const void* x, void* dw, float* part, hipStream_t s) {
-  const LinOp<T> og{(const T*)gz, d->n, d->n, d->rows}, ox{(const T*)x, d->ldx, d->k, d->rows};
-  const LinEpi<T> ep{nullptr, nullptr, nullptr, (T*)dw, nullptr, LIN_NONE};
-  return lin_product<T, true, true>(og, ox, ep, part, s);
-}
-
-template <typename T>
-static int lin_act_bwd_run(const vfd_linear_desc* d, const void* g, const void* z, void* gz, void* db, float* part, hipStream_t s) {
-  const int strips = lin_strips(d->rows, d->n, LinT<T>::VE);
-  const dim3 grid(cdiv(d->n, 64 * LinT<T>::VE), strips);
-  lin_with_act(d->act, [&](auto act) {
-    lin_act_bwd_k<T, act()><<<grid, 256, 0, s>>>((const T*)g, (const T*)z, (T*)gz, db ? part : nullptr, d->rows, d->n);
-    return 0;
-  });
-  if (db) col_sums_k<T><<<cdiv(d->n, COLSUM_COLS), 1024, 0, s>>>(part, strips, d->n, d->n, (T*)db, nullptr);
-  return fail_launch("linear_bwd activation");
-}
-
-template <typename T>
-static int lin_bwd_run(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
-                       void* dw, void* db, float* ws, hipStream_t s) {
-  if (d->act != LIN_NONE || db)
-    if (int e = lin_act_bwd_run<T>(d, g, z, gz, db, ws, s)) return e;
-  if (d->act == LIN_NONE) gz = const_cast<void*>(g);
-  if (dx)
-    if (int e = lin_dgrad_run<T>(d, gz, w, dx, ws, s)) return e;
-  return dw ? lin_wgrad_run<T>(d, gz, x, dw, ws, s) : VFD_OK;
+static int lin_bwd_run(const vfd_linear_desc* d, const T* g, const T* z, const T* w, const T* x, T* dx, T* dw, T* db, char* ws,
+                       hipStream_t s) {
+  const LinBwdPlan p = lin_bwd_plan<T>(d, g, w, x, dx != nullptr, dw != nullptr);
+  float* part = (float*)(ws + p.at_part);
+  const LinEpi<T> plain{nullptr, nullptr, nullptr, nullptr, nullptr, LIN_NONE};
+  if (p.gz || db) {
+    T* gz = p.gz ? (T*)(ws + p.at_gz) : nullptr;
+    const int strips = lin_strips(d->rows, d->n, LinT<T>::VE);
+    const dim3 grid(cdiv(d->n, 64 * LinT<T>::VE), strips);
+    lin_with_act(d->act, [&](auto act) {
+      lin_act_bwd_k<T, act()><<<grid, 256, 0, s>>>(g, z, gz, p.ldg, db ? part : nullptr, d->rows, d->n);
+      return 0;
+    });
+    if (db) col_sums_k<T><<<cdiv(d->n, COLSUM_COLS), 1024, 0, s>>>(part, strips, d->n, d->n, db, nullptr);
+    if (int e = fail_launch("linear_bwd activation")) return e;
+    if (gz) g = gz;
+  }
+  if (dx) {
+    if (p.w) {
+      T* c = (T*)(ws + p.at_w);
+      lin_pack(w, d->k, c, p.ldw, d->n, d->k, s);
+      w = c;
+    }
+    LinEpi<T> ep = plain;
+    ep.y = dx;
+    const LinOp<T> og{g, p.ldg, d->rows, d->n}, ow{w, p.ldw, d->k, d->n};
+    if (int e = lin_product<T, false, true>(og, ow, ep, part, s)) return e;
+  }
+  if (dw) {
+    if (p.x) {
+      T* c = (T*)(ws + p.at_x);
+      lin_pack(x, d->ldx, c, p.ldx, d->rows, d->k, s);
+      x = c;
+    }
+    LinEpi<T> ep = plain;
+    ep.y = dw;
+    const LinOp<T> og{g, p.ldg, d->n, d->rows}, ox{x, p.ldx, d->k, d->rows};
+    if (int e = lin_product<T, true, true>(og, ox, ep, part, s)) return e;
+  }
+  return VFD_OK;
 }
 
 }  // namespace vfd
@@ -979,13 +1039,13 @@ int vfd_linear_fwd(const vfd_linear_desc* d, const void* x, const void* w, const
   return (d->dtype ? lin_fwd_run<__bf16> : lin_fwd_run<float>)(d, x, w, bias, res, y, z, (float*)workspace, s);
 }
 
-size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d) {
+size_t vfd_linear_bwd_workspace(const vfd_linear_desc* d, const void* g, const void* w, const void* x, int dx, int dw) {
   if (lin_check("linear", d) != VFD_OK || d->rows == 0) return 0;
-  return d->dtype ? lin_bwd_ws<__bf16>(d) : lin_bwd_ws<float>(d);
+  return (d->dtype ? lin_bwd_plan<__bf16> : lin_bwd_plan<float>)(d, g, w, x, dx != 0, dw != 0).bytes;
 }
 
-int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* gz, void* dx,
-                   void* dw, void* db, void* workspace, size_t ws_bytes, void* stream) {
+int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const void* w, const void* x, void* dx, void* dw,
+                   void* db, void* workspace, size_t ws_bytes, void* stream) {
   if (int e = lin_check("linear_bwd", d)) return e;
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof(K_LINEAR_BWD, s);
@@ -996,9 +1056,14 @@ int vfd_linear_bwd(const vfd_linear_desc* d, const void* g, const void* z, const
     return fail_launch("linear_bwd");
   }
   if (!dx && !dw && !db) return VFD_OK;
-  VFD_REQUIRE(g && (d->act == LIN_NONE || (z && gz)) && (!dx || w) && (!dw || x), "linear_bwd: null tensor");
-  VFD_REQUIRE(workspace && ws_bytes >= vfd_linear_bwd_workspace(d), "linear_bwd: workspace too small");
-  return (d->dtype ? lin_bwd_run<__bf16> : lin_bwd_run<float>)(d, g, z, w, x, gz, dx, dw, db, (float*)workspace, s);
+  VFD_REQUIRE(g && (d->act == LIN_NONE || z) && (!dx || w) && (!dw || x), "linear_bwd: null tensor");
+  VFD_REQUIRE(workspace && ws_bytes >= vfd_linear_bwd_workspace(d, g, w, x, dx != nullptr, dw != nullptr),
+              "linear_bwd: workspace too small");
+  if (d->dtype)
+    return lin_bwd_run<__bf16>(d, (const __bf16*)g, (const __bf16*)z, (const __bf16*)w, (const __bf16*)x, (__bf16*)dx, (__bf16*)dw,
+                               (__bf16*)db, (char*)workspace, s);
+  return lin_bwd_run<float>(d, (const float*)g, (const float*)z, (const float*)w, (const float*)x, (float*)dx, (float*)dw, (float*)db,
+                            (char*)workspace, s);
 }
 
 }  // extern "C"

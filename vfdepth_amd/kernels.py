@@ -2274,12 +2274,11 @@ class LinearAct(torch.autograd.Function):
         dx = torch.empty((*g.shape[:-1], d.k), dtype=g.dtype, device=g.device) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty(d.n, dtype=g.dtype, device=g.device) if need_b else None
-        nws = lib.vfd_linear_bwd_workspace(d)
-        at = -(-nws // 256) * 256                       # the gradient behind the activation lies behind the workspace
-        ws = _ws(at + (g.numel() * g.element_size() if d.act else 0), g.device)
-        p = ws.data_ptr()
-        L.check(lib.vfd_linear_bwd(d, g.data_ptr(), L.ptr(z), weight.data_ptr(), x.data_ptr(), p + at, L.ptr(dx), L.ptr(dw),
-                                   L.ptr(db), p, nws, L.stream()), 'linear_bwd')
+        pg, pw, px = g.data_ptr(), weight.data_ptr(), x.data_ptr()
+        nws = lib.vfd_linear_bwd_workspace(d, pg, pw, px, need_x, need_w)
+        ws = _ws(nws, g.device)
+        L.check(lib.vfd_linear_bwd(d, pg, L.ptr(z), pw, px, L.ptr(dx), L.ptr(dw), L.ptr(db), ws.data_ptr(), nws, L.stream()),
+                'linear_bwd')
         if L.PROF_ON:
             L.ALG_BYTES['linear_bwd'] += x.element_size() * (g.numel() * (1 + 2 * (d.act != 0)) + (need_x + need_w)
                                                              * (g.numel() + x.numel() + weight.numel()))
