@@ -2303,58 +2303,51 @@ def _dense(t):
     return True
 
 
-_dtype_of, _layout_of, _shape_of = (operator.attrgetter(a) for a in ('dtype', 'layout', 'shape'))
+_dtype_of, _shape_of = operator.attrgetter('dtype'), operator.attrgetter('shape')
 
 
 def _clip_list(tensors, what):
-    """Checked list of gradient tensors: strided fp32 / bf16 tensors on the current HIP device."""
+    """A list of gradient tensors, strided fp32 / bf16 on the current HIP device, with what the kernels' table holds of
+    each: its address, length and type code."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    # whole-list passes (a model has hundreds of gradients, and the kernels take tens of microseconds), tensor by tensor
+    # whole-list passes (a model has hundreds of gradients, and the kernels take tens of microseconds); tensor by tensor
     # only to name the one that does not fit
     try:
-        if (set(map(torch.Tensor.get_device, tensors)) <= {torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None}
-                and set(map(_dtype_of, tensors)) <= _CLIP_DTYPES.keys() and set(map(_layout_of, tensors)) <= {torch.strided}):
-            return tensors
-    except TypeError:                       # something that is no tensor
+        kinds = set(map(_dtype_of, tensors))
+        if (kinds <= _CLIP_DTYPES.keys() and set(map(torch.Tensor.get_device, tensors))
+                <= {torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None}):
+            ptrs = array.array('Q', map(torch.Tensor.data_ptr, tensors))             # (none of a sparse tensor)
+            codes = (bytes([_CLIP_DTYPES[k] for k in kinds]) * len(tensors) if len(kinds) == 1 else
+                     bytes([_CLIP_DTYPES[t.dtype] for t in tensors]))
+            return tensors, ptrs, array.array('q', map(torch.Tensor.numel, tensors)), codes
+    except (AttributeError, TypeError, RuntimeError):       # something that is no tensor, or has no memory of its own
         pass
     for t in tensors:
         _check_device(t, what)
         if t.dtype not in _CLIP_DTYPES or t.layout is not torch.strided:
             raise RuntimeError(f'{what}: strided fp32 or bf16 tensors, got {t.dtype} ({t.layout})')
-    return tensors
+    raise RuntimeError(f'{what}: a tensor without memory of its own')
 
 
-def _clip_codes(tensors):
-    kinds = set(map(_dtype_of, tensors))
-    if len(kinds) == 1:
-        return bytes([_CLIP_DTYPES[kinds.pop()]]) * len(tensors)
-    return bytes([_CLIP_DTYPES[t.dtype] for t in tensors])
-
-
-def _clip_call(fn, tensors, norm_type, extra=(), outs=None):
-    """One C call over a list: (pointers, lengths, types) as host arrays, the norm and the partials' workspace."""
+def _clip_call(fn, listed, norm_type, extra=(), outs=None):
+    """One C call over a list: the norm, and the partials' workspace."""
     lib = L.load()
     if norm_type not in (2, math.inf):
         raise ValueError(f'{fn}: norm_type 2 or inf, got {norm_type!r}')
+    tensors, ptrs, numel, codes = listed
     n = len(tensors)
     device = tensors[0].device if n else torch.device('cuda', torch.cuda.current_device())
-    ptrs = array.array('Q', map(torch.Tensor.data_ptr, tensors))
-    numel = array.array('q', map(torch.Tensor.numel, tensors))
     at = lambda a: a.buffer_info()[0]  # noqa: E731
     norm = torch.empty((), dtype=torch.float32, device=device)
     nws = lib.vfd_grad_norm_workspace(n, at(numel))
     ws = _ws(nws, device)
-    args = [n, at(ptrs), at(numel), _clip_codes(tensors), int(norm_type == math.inf), *extra]
+    args = [n, at(ptrs), at(numel), codes, int(norm_type == math.inf), *extra]
     if fn == 'clip_grads':
-        if outs is None:
-            args += [None, None]
-        else:
-            optrs = array.array('Q', map(torch.Tensor.data_ptr, outs))
-            args += [at(optrs), _clip_codes(outs)]
+        args += [None, None] if outs is None else [at(outs[1]), outs[3]]
     L.check(getattr(lib, 'vfd_' + fn)(*args, norm.data_ptr(), ws.data_ptr(), nws, L.stream()), fn)
     if L.PROF_ON:                            # compulsory: the gradients once, the clipped ones once
         L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in tensors)
-        L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in (outs or ()))
+        L.ALG_BYTES['grad_clip'] += sum(t.numel() * t.element_size() for t in (outs[0] if outs else ()))
     return norm
 
 
@@ -2363,8 +2356,10 @@ def grad_norm(grads, norm_type=2.0):
     """Global norm of a list of gradient tensors (fp32 / bf16, mixed at will) as a 0-d fp32 tensor on the device:
     sqrt of the sum of all squares, or the largest magnitude for norm_type inf.  Summed in fp64 in a fixed order;
     nothing waits on the host.  An empty list gives 0."""
-    tensors = _clip_list(grads, 'grad_norm')
-    return _clip_call('grad_norm', [t if _dense(t) else t.contiguous() for t in tensors], norm_type)
+    listed = _clip_list(grads, 'grad_norm')
+    if not all(map(torch.Tensor.is_contiguous, listed[0])):
+        listed = _clip_list([t if _dense(t) else t.contiguous() for t in listed[0]], 'grad_norm')
+    return _clip_call('grad_norm', listed, norm_type)
 
 
 @torch.no_grad()
@@ -2375,32 +2370,34 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     are.  max_norm is a host number (a captured graph keeps it).  A NaN norm makes every gradient NaN, an infinite
     one makes finite gradients 0, as torch.nn.utils.clip_grad_norm_.  Tensors that are written must not share memory
     with each other or, with `out`, with a gradient."""
-    tensors = _clip_list(grads, 'clip_grads')
+    listed = _clip_list(grads, 'clip_grads')
+    tensors = listed[0]
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f'clip_grads: max_norm must be a number >= 0, got {max_norm}')
+    plain = all(map(torch.Tensor.is_contiguous, tensors))
     if out is None:
-        if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(map(_dense, tensors)):
+        if not plain and not all(map(_dense, tensors)):
             raise ValueError('clip_grads: a gradient that is not stored densely is clipped into `out`, not in place')
-        norm = _clip_call('clip_grads', tensors, norm_type, (max_norm,))
+        norm = _clip_call('clip_grads', listed, norm_type, (max_norm,))
     else:
         outs = _clip_list(out, 'clip_grads out')
-        if len(outs) != len(tensors):
-            raise ValueError(f'clip_grads: {len(tensors)} gradients, {len(outs)} outputs')
-        work = tensors
-        if not (all(map(torch.Tensor.is_contiguous, tensors)) and all(map(torch.Tensor.is_contiguous, outs))
-                and all(map(operator.eq, map(_shape_of, tensors), map(_shape_of, outs)))):
+        if len(outs[0]) != len(tensors):
+            raise ValueError(f'clip_grads: {len(tensors)} gradients, {len(outs[0])} outputs')
+        if not (plain and all(map(torch.Tensor.is_contiguous, outs[0]))
+                and all(map(operator.eq, map(_shape_of, tensors), map(_shape_of, outs[0])))):
             work = []
-        for t, o in zip(tensors, outs) if work is not tensors else ():
-            if t.shape != o.shape:
-                raise ValueError(f'clip_grads: gradient {tuple(t.shape)} into output {tuple(o.shape)}')
-            if not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _dense(t)):
-                if not o.is_contiguous():
-                    raise ValueError('clip_grads: an output is contiguous or laid out as its gradient')
-                t = t.contiguous()
-            work.append(t)
-        norm = _clip_call('clip_grads', work, norm_type, (max_norm,), outs)
-        tensors = outs
+            for t, o in zip(tensors, outs[0]):
+                if t.shape != o.shape:
+                    raise ValueError(f'clip_grads: gradient {tuple(t.shape)} into output {tuple(o.shape)}')
+                if not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _dense(t)):
+                    if not o.is_contiguous():
+                        raise ValueError('clip_grads: an output is contiguous or laid out as its gradient')
+                    t = t.contiguous()
+                work.append(t)
+            listed = _clip_list(work, 'clip_grads')
+        norm = _clip_call('clip_grads', listed, norm_type, (max_norm,), outs)
+        tensors = outs[0]
     try:
         torch.autograd.graph.increment_version(tensors)
     except RuntimeError:                    # inference tensors have no version
