@@ -139,13 +139,26 @@ def test_widths(C, dtype):
 
 @gpu
 @pytest.mark.parametrize('dtype', [F32, BF16])
-@pytest.mark.parametrize('rows,C', [(2, 64), (4097, 24), (30001, 64), (9000, 256), (5761, 1021), (1500, 4096), (700, 9001)])
+@pytest.mark.parametrize('rows,C', [(2, 64), (4097, 24), (30001, 64), (9000, 256), (5761, 1021), (1500, 4096), (700, 9001), (150, 40001)])
 def test_many_rows(rows, C, dtype):
     x, w, b, g = (t.cuda() for t in _case(rows, C, dtype, seed=rows))
     y, grads = _run(x, w, b, g)
     _check((y, *grads), *_oracle(x, w, b, g))
     y2, grads2 = _run(x, w, b, g)                            # fixed order of every sum
     assert torch.equal(y, y2) and all(torch.equal(a, c) for a, c in zip(grads, grads2))
+
+
+@gpu
+def test_inference_keeps_nothing():
+    from vfdepth_amd import layers
+    ln, x = torch.nn.LayerNorm(8).cuda(), torch.randn(1 << 20, 8, device='cuda')
+    want = layers.layer_norm(ln, x).detach()
+    with torch.no_grad():
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = layers.layer_norm(ln, x)
+        assert torch.cuda.max_memory_allocated() - base <= 1.1 * y.numel() * 4
+    assert not y.requires_grad and torch.equal(y, want)
 
 
 @gpu

@@ -212,6 +212,7 @@ def test_activations(act, bias, residual, dtype):
     from vfdepth_amd import kernels as KN
     with torch.no_grad():                                        # without a pre-activation to keep: the same bits
         assert torch.equal(KN.LinearAct.apply(*args[:4], act), out[0])
+        assert torch.equal(KN.LinearAct.infer(*args[:4], act), out[0])
 
 
 @gpu
@@ -318,6 +319,45 @@ def test_non_finite_rows_stay_in_their_rows(dtype):
     xn = x.clone()
     xn[3, 4] = math.nan
     assert torch.isnan(KN.LinearAct.apply(xn, w, b, None, 'relu')[3]).all()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_relu_stops_non_finite_gradients(dtype):
+    x, w, b, _, g = _case(70, 24, 40, dtype, seed=9)
+    with torch.no_grad():
+        off = (x.float() @ w.float().t() + b.float() < -0.05)
+    clean, bad = g.masked_fill(off, 0), g.masked_fill(off, math.inf)
+    bad[1::2] = g[1::2].masked_fill(off[1::2], math.nan)
+    outs = [_run(x.detach(), w.detach(), b.detach(), None, t, 'relu') for t in (clean, bad)]
+    for a, c in zip(*outs):
+        assert a is None or torch.equal(a, c)
+
+
+@gpu
+def test_inference_keeps_nothing():
+    """Without a graph neither a pre-activation is written nor its memory taken, though the weights want gradients."""
+    from vfdepth_amd import layers
+    lin = torch.nn.Linear(64, 4096).cuda()
+    x = torch.randn(4096, 64, device='cuda')
+    want = layers.linear_act(lin, x, 'gelu').detach()
+    with torch.no_grad():
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = layers.linear_act(lin, x, 'gelu')
+        assert torch.cuda.max_memory_allocated() - base <= 1.25 * y.numel() * 4
+    assert not y.requires_grad and torch.equal(y, want)
+
+
+@gpu
+def test_very_wide_output():
+    """A row of x against more weights than one launch of the few-rows form has blocks for: K = 1, so a product is exact to
+    its rounding."""
+    from vfdepth_amd import kernels as KN
+    w = torch.randn((1 << 26) + 133, 1, device='cuda').bfloat16()
+    x = torch.tensor([[1.5], [-3.0]], device='cuda').bfloat16()
+    y = KN.LinearAct.infer(x, w, None, None, 'none')
+    assert torch.equal(y, (x.float() * w.float().t()).bfloat16())
 
 
 @gpu

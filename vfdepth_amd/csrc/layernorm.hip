@@ -10,6 +10,7 @@
 // pass over registers, not over memory).  Blocks walk over rows and load the next row while they work on this one.  The
 // backward's column sums stay in registers over all rows of a block; blocks leave one partial row each, which a second
 // launch adds in block order: no atomics, the same bits every time.
+#include <algorithm>
 #include <type_traits>
 
 #include "vfd_common.h"
@@ -361,7 +362,7 @@ template <typename T>
 static int ln_parts(int rows, int C) {
   return ln_pick<T>(C, [&](auto l, auto w, auto nv) {
     if constexpr (decltype(l)::value == 0)
-      return rows < 128 ? rows : 128;
+      return std::max(1, std::min({rows, 128, (1 << 22) / C}));      // (partials of at most 32 MB up to 2^22 columns)
     else
       return ln_bwd_blocks(rows, LnGroup<T, l(), w(), nv()>::RB, w(), LnGroup<T, l(), w(), nv()>::E);
   });

@@ -57,7 +57,6 @@ __device__ __forceinline__ float lin_act(float z) {
 
 template <int ACT>
 __device__ __forceinline__ float lin_slope(float z) {
-  if constexpr (ACT == LIN_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == LIN_LRELU) return z > 0.f ? 1.f : LIN_SLOPE;
   if constexpr (ACT == LIN_ELU) return z > 0.f ? 1.f : lin_exp(z);
   if constexpr (ACT == LIN_GELU) {
@@ -70,6 +69,13 @@ __device__ __forceinline__ float lin_slope(float z) {
     return s * fmaf(z, 1.f - s, 1.f);
   }
   return 1.f;
+}
+
+// g act'(z).  Where ReLU lets nothing through, an infinite or NaN g does not pass either.
+template <int ACT>
+__device__ __forceinline__ float lin_back(float g, float z) {
+  if constexpr (ACT == LIN_RELU) return z <= 0.f ? 0.f : g;
+  return g * lin_slope<ACT>(z);
 }
 
 template <typename F>
@@ -692,7 +698,7 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
         vec o;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (ACT != LIN_NONE) f[u][j] *= lin_slope<ACT>(zf[u][j]);
+          if (ACT != LIN_NONE) f[u][j] = lin_back<ACT>(f[u][j], zf[u][j]);
           s[j] += f[u][j];
           o[j] = (T)f[u][j];
         }
@@ -899,7 +905,8 @@ static int lin_strips(int M, int N, int V) {               // row blocks of lin_
   return need < most ? need : most;
 }
 
-static bool lin_is_thin(const vfd_linear_desc* d) { return d->rows <= LIN_THIN; }
+// (a launch holds under 2^32 threads)
+static bool lin_is_thin(const vfd_linear_desc* d) { return d->rows <= LIN_THIN && d->n <= (1 << 26); }
 
 template <typename T>
 static size_t lin_fwd_ws(const vfd_linear_desc* d) {
@@ -943,8 +950,8 @@ static int lin_check(const char* what, const vfd_linear_desc* d) {
                   d->n <= VFD_LINEAR_MAX && d->ldx >= d->k && d->act >= 0 && d->act < LIN_ACTS && (d->dtype == 0 || d->dtype == 1),
               "%s: bad descriptor", what);
   const long long T = 128;
-  VFD_REQUIRE(((long long)d->rows / T + 1) * (d->n / T + 1) < (1 << 30) && ((long long)d->rows / T + 1) * (d->k / T + 1) < (1 << 30) &&
-                  ((long long)d->n / T + 1) * (d->k / T + 1) < (1 << 30),
+  VFD_REQUIRE(((long long)d->rows / T + 1) * (d->n / T + 1) < (1 << 24) && ((long long)d->rows / T + 1) * (d->k / T + 1) < (1 << 24) &&
+                  ((long long)d->n / T + 1) * (d->k / T + 1) < (1 << 24),
               "%s: too many tiles", what);
   return VFD_OK;
 }

@@ -2169,6 +2169,17 @@ class LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
+        y, ctx.d, *saved = LayerNorm._run(x, weight, bias, eps, any(ctx.needs_input_grad))
+        ctx.save_for_backward(*saved)
+        return y
+
+    @staticmethod
+    def infer(x, weight, bias, eps):
+        """The forward without a graph: no statistics are kept."""
+        return LayerNorm._run(x, weight, bias, eps, False)[0]
+
+    @staticmethod
+    def _run(x, weight, bias, eps, keep):
         lib = L.load()
         _check_device(x, 'layer norm input')
         C = x.shape[-1] if x.dim() else 0
@@ -2182,7 +2193,7 @@ class LayerNorm(torch.autograd.Function):
         d = L.NormDesc(rows, C, ldx, eps, _dt(x))
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         stats = m = r = None
-        if any(ctx.needs_input_grad):
+        if keep:
             stats = torch.empty(2 * rows, dtype=torch.float32, device=y.device)      # means, then 1 / deviations
             m = stats.data_ptr()
             r = m + 4 * rows
@@ -2190,9 +2201,7 @@ class LayerNorm(torch.autograd.Function):
                 'layer_norm_fwd')
         if L.PROF_ON:
             L.ALG_BYTES['layer_norm_fwd'] += 2 * x.numel() * x.element_size()
-        ctx.d = d
-        ctx.save_for_backward(x2, weight, stats)
-        return y
+        return y, d, x2, weight, stats
 
     @_once
     def backward(ctx, g):
@@ -2228,6 +2237,17 @@ class LinearAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
+        y, ctx.d, *saved = LinearAct._run(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(*saved)
+        return y
+
+    @staticmethod
+    def infer(x, weight, bias, residual, act):
+        """The forward without a graph: no pre-activation is kept."""
+        return LinearAct._run(x, weight, bias, residual, act, False)[0]
+
+    @staticmethod
+    def _run(x, weight, bias, residual, act, keep):
         lib = L.load()
         _check_device(x, 'linear input')
         if act not in L.LINEAR_ACTS:
@@ -2247,7 +2267,7 @@ class LinearAct(torch.autograd.Function):
         d = L.LinearDesc(rows, K, N, L.LINEAR_ACTS[act], ldx, code)
         y = torch.empty(shape, dtype=dtype, device=x.device)
         z = None
-        if d.act and any(ctx.needs_input_grad[:3]):
+        if d.act and keep:
             z = torch.empty_like(y)
         ws, nws = None, lib.vfd_linear_fwd_workspace(d)
         if nws:
@@ -2257,9 +2277,7 @@ class LinearAct(torch.autograd.Function):
         if L.PROF_ON:
             L.ALG_BYTES['linear_fwd'] += x.element_size() * (x.numel() + weight.numel() + y.numel()
                                                              * (1 + (z is not None) + (residual is not None)))
-        ctx.d = d
-        ctx.save_for_backward(x2, weight, z)
-        return y
+        return y, d, x2, weight, z
 
     @_once
     def backward(ctx, g):

@@ -155,7 +155,7 @@ def layer_norm(ln, x):
             and x.shape[-1] == ln.normalized_shape[0]):
         from . import kernels as KN
         w, b = (p if p is None or p.dtype == torch.float32 else p.float() for p in (ln.weight, ln.bias))
-        return KN.LayerNorm.apply(x, w, b, ln.eps)
+        return (KN.LayerNorm.apply if torch.is_grad_enabled() else KN.LayerNorm.infer)(x, w, b, ln.eps)
     return ln(x)
 
 
@@ -189,10 +189,11 @@ def linear_act(lin, x, act='none', residual=None):
     w, b = lin.weight, lin.bias
     if torch.is_autocast_enabled('cuda'):
         x, w, b, residual = (None if t is None else t.to(dt) for t in (x, w, b, residual))
+    run = KN.LinearAct.apply if torch.is_grad_enabled() else KN.LinearAct.infer
     if not conv:
-        return KN.LinearAct.apply(x, w, b, residual, act)
+        return run(x, w, b, residual, act)
     r = residual.permute(0, 2, 3, 1) if residual is not None else None
-    return KN.LinearAct.apply(x.permute(0, 2, 3, 1), w.flatten(1), b, r, act).permute(0, 3, 1, 2)
+    return run(x.permute(0, 2, 3, 1), w.flatten(1), b, r, act).permute(0, 3, 1, 2)
 
 
 class BasicBlock(nn.Module):
