@@ -254,25 +254,62 @@ __global__ __launch_bounds__((LnGroup<T, L, W, NV>::BLOCK)) void ln_bwd_k(
   }
 }
 
-// Rows too wide for a block's registers (over 8192 values: sixteen waves of 16 values a lane would spill): the row is read again for each pass (from cache), a block a row.
+// Rows too wide for a block's registers (over 8192 values: sixteen waves of 16 values a lane would spill): a block a row,
+// read again for each pass (from cache), 16 bytes a thread at a time.  4096 x 12 288 bf16: 49 us forward, 186 with its
+// backward; 169 and 400 with blocks of 256 and a value a thread at a time.
+constexpr int LN_WIDE = 1024;
+template <typename T, typename F>
+__device__ __forceinline__ void ln_each(int C, F f) {       // f(first column, its values) over this thread's vectors of a row
+  constexpr int V = LnV<T>::V;
+  for (int c = (int)threadIdx.x * V; c < C; c += LN_WIDE * V) f(c, min(C - c, V));
+}
+
+// A vector's parameters from column c on; null: `other`
+template <int V>
+__device__ __forceinline__ void ln_wide_params(const float* __restrict__ p, int c, int cnt, float other, float (&f)[V]) {
+#pragma unroll
+  for (int h = 0; h < V; h += 4) {
+    LnV<float>::vec v = {other, other, other, other};
+    if (p != nullptr) v = ln_load(p + c + h, cnt - h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[h + j] = v[j];
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void ln_fwd_wide_k(const T* __restrict__ x, long long ldx, const float* __restrict__ w,
-                                                     const float* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
-                                                     float* __restrict__ rstd, int rows, int C, float eps) {
-  __shared__ float lds[4];
+__global__ __launch_bounds__(LN_WIDE) void ln_fwd_wide_k(const T* __restrict__ x, long long ldx, const float* __restrict__ w,
+                                                         const float* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
+                                                         float* __restrict__ rstd, int rows, int C, float eps) {
+  constexpr int V = LnV<T>::V, W = LN_WIDE / 64;
+  __shared__ float lds[2 * W];
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
     float s = 0.f;
-    for (int c = threadIdx.x; c < C; c += 256) s += ld1(xr + c);
-    const float m = block_sum_all(s, lds) / (float)C;
+    ln_each<T>(C, [&](int c, int cnt) {
+      const auto v = ln_load(xr + c, cnt);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += (float)v[j];
+    });
+    const float m = ln_sum<64, W>(s, lds, 0) / (float)C;
     s = 0.f;
-    for (int c = threadIdx.x; c < C; c += 256) {
-      const float e = ld1(xr + c) - m;
-      s = fmaf(e, e, s);
-    }
-    const float r = 1.f / sqrtf(block_sum_all(s, lds) / (float)C + eps);
-    for (int c = threadIdx.x; c < C; c += 256)
-      st1(y + row * C + c, fmaf((ld1(xr + c) - m) * r, w ? w[c] : 1.f, b ? b[c] : 0.f));
+    ln_each<T>(C, [&](int c, int cnt) {
+      const auto v = ln_load(xr + c, cnt);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float e = j < cnt ? (float)v[j] - m : 0.f;
+        s = fmaf(e, e, s);
+      }
+    });
+    const float r = 1.f / sqrtf(ln_sum<64, W>(s, lds, 1) / (float)C + eps);
+    ln_each<T>(C, [&](int c, int cnt) {
+      const auto v = ln_load(xr + c, cnt);
+      float f[V], wv[V], bv[V];
+      ln_wide_params(w, c, cnt, 1.f, wv);
+      ln_wide_params(b, c, cnt, 0.f, bv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = fmaf(((float)v[j] - m) * r, wv[j], bv[j]);
+      ln_store(y + row * C + c, f, cnt);
+    });
     if (mean != nullptr && threadIdx.x == 0) {
       mean[row] = m;
       rstd[row] = r;
@@ -281,23 +318,36 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_k(const T* __restrict__ x, lo
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ln_bwd_wide_k(const T* __restrict__ g, const T* __restrict__ x, long long ldx,
-                                                     const float* __restrict__ w, const float* __restrict__ mean,
-                                                     const float* __restrict__ rstd, T* __restrict__ dx, int rows, int C) {
-  __shared__ float lds[4];
+__global__ __launch_bounds__(LN_WIDE) void ln_bwd_wide_k(const T* __restrict__ g, const T* __restrict__ x, long long ldx,
+                                                         const float* __restrict__ w, const float* __restrict__ mean,
+                                                         const float* __restrict__ rstd, T* __restrict__ dx, int rows, int C) {
+  constexpr int V = LnV<T>::V, W = LN_WIDE / 64;
+  __shared__ float lds[2 * W];
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T *xr = x + row * ldx, *gr = g + row * C;
     const float m = mean[row], r = rstd[row];
     float s1 = 0.f, s2 = 0.f;
-    for (int c = threadIdx.x; c < C; c += 256) {
-      const float gw = ld1(gr + c) * (w ? w[c] : 1.f);
-      s1 += gw;
-      s2 = fmaf(gw, (ld1(xr + c) - m) * r, s2);
-    }
-    s1 = block_sum_all(s1, lds) / (float)C;
-    s2 = block_sum_all(s2, lds) / (float)C;
-    for (int c = threadIdx.x; c < C; c += 256)
-      st1(dx + row * C + c, r * (fmaf(ld1(gr + c), w ? w[c] : 1.f, -s1) - (ld1(xr + c) - m) * r * s2));
+    ln_each<T>(C, [&](int c, int cnt) {
+      const auto xv = ln_load(xr + c, cnt), gv = ln_load(gr + c, cnt);
+      float wv[V];
+      ln_wide_params(w, c, cnt, 1.f, wv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float gw = j < cnt ? (float)gv[j] * wv[j] : 0.f;
+        s1 += gw;
+        s2 = fmaf(gw, j < cnt ? ((float)xv[j] - m) * r : 0.f, s2);
+      }
+    });
+    s1 = ln_sum<64, W>(s1, lds, 0) / (float)C;
+    s2 = ln_sum<64, W>(s2, lds, 1) / (float)C;
+    ln_each<T>(C, [&](int c, int cnt) {
+      const auto xv = ln_load(xr + c, cnt), gv = ln_load(gr + c, cnt);
+      float f[V], wv[V];
+      ln_wide_params(w, c, cnt, 1.f, wv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = r * (fmaf((float)gv[j], wv[j], -s1) - ((float)xv[j] - m) * r * s2);
+      ln_store(dx + row * C + c, f, cnt);
+    });
   }
 }
 
@@ -307,11 +357,22 @@ __global__ __launch_bounds__(256) void ln_cols_wide_k(const T* __restrict__ g, c
                                                       float* __restrict__ part, int rows, int C) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= C) return;
+  constexpr int U = 4;                                       // rows in flight
   float dw = 0.f, db = 0.f;
-  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float gv = ld1(g + row * C + c);
-    dw = fmaf(gv, (ld1(x + row * ldx + c) - mean[row]) * rstd[row], dw);
-    db += gv;
+  for (long long row = blockIdx.y; row < rows; row += (long long)U * gridDim.y) {
+    float gv[U], h[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long r = row + u * (long long)gridDim.y, q = r < rows ? r : rows - 1;
+      gv[u] = ld1(g + q * C + c);
+      h[u] = (ld1(x + q * ldx + c) - mean[q]) * rstd[q];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (row + u * (long long)gridDim.y < rows) {
+        dw = fmaf(gv[u], h[u], dw);
+        db += gv[u];
+      }
   }
   part[(size_t)blockIdx.y * 2 * C + c] = dw;
   part[(size_t)blockIdx.y * 2 * C + C + c] = db;
@@ -374,7 +435,7 @@ static int ln_fwd_run(const vfd_norm_desc* d, const void* x, const float* w, con
   return ln_pick<T>(d->cols, [&](auto l, auto wv, auto nv) {
     if constexpr (decltype(l)::value == 0) {
       const int grid = d->rows < LN_FWD_GRID ? d->rows : LN_FWD_GRID;
-      ln_fwd_wide_k<T><<<grid, 256, 0, s>>>((const T*)x, d->ldx, w, b, (T*)y, mean, rstd, d->rows, d->cols, d->eps);
+      ln_fwd_wide_k<T><<<grid, LN_WIDE, 0, s>>>((const T*)x, d->ldx, w, b, (T*)y, mean, rstd, d->rows, d->cols, d->eps);
     } else {
       typedef LnGroup<T, l(), wv(), nv()> Gr;
       const int need = (d->rows + Gr::RB - 1) / Gr::RB, grid = need < LN_FWD_GRID ? need : LN_FWD_GRID;
@@ -392,7 +453,7 @@ static int ln_bwd_run(const vfd_norm_desc* d, const void* g, const void* x, cons
   const int e = ln_pick<T>(d->cols, [&](auto l, auto wv, auto nv) {
     if constexpr (decltype(l)::value == 0) {
       if (dx)
-        ln_bwd_wide_k<T><<<d->rows < LN_FWD_GRID ? d->rows : LN_FWD_GRID, 256, 0, s>>>((const T*)g, (const T*)x, d->ldx, w, mean,
+        ln_bwd_wide_k<T><<<d->rows < LN_FWD_GRID ? d->rows : LN_FWD_GRID, LN_WIDE, 0, s>>>((const T*)g, (const T*)x, d->ldx, w, mean,
                                                                               rstd, (T*)dx, d->rows, d->cols);
       if (cols)
         ln_cols_wide_k<T><<<dim3(cdiv(d->cols, 256), nb), 256, 0, s>>>((const T*)g, (const T*)x, d->ldx, mean, rstd, part,
