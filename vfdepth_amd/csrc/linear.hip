@@ -316,12 +316,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void lin_tile_k(LinOp<T> x, LinO
   constexpr int BK = TX::BK, KS = RB / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   constexpr int STAGE = (BM + BN) * RB, LOADS = TX::NCH + TW::NCH;
-  // tiles of one XCD (every eighth workgroup) are consecutive: column groups of 8 row tiles, splits outermost
+  // tiles of one XCD (every eighth workgroup) are consecutive: column groups of 4 row tiles, splits outermost
+  // (of 8: 16 384 x 2048 x 8192 bf16 461 us forward, 514 data gradient; 446 and 495 with 4)
   const int total = tm * tn * splits, xcd = blockIdx.x % 8, per = total / 8, rest = total % 8;
   int t = xcd * per + min(xcd, rest) + blockIdx.x / 8;
   const int split = t / (tm * tn);
   t -= split * tm * tn;
-  constexpr int GM = 8;
+  constexpr int GM = 4;
   const int group = t / (GM * tn), g0 = group * GM, gm = min(GM, tm - g0);
   t -= group * GM * tn;
   const int m0 = (g0 + t % gm) * BM, n0 = (t / gm) * BN;
