@@ -228,6 +228,20 @@ def test_large_product(dtype):
         _check(_run(*args, 'none'), *_oracle(*args, 'none'))
 
 
+# Ragged sizes at which each tile form and split is taken, in either type (forward, data gradient or weight gradient)
+FORMS = [(12687, 9, 193), (17993, 8, 65), (16825, 143, 8), (12431, 216, 528), (18686, 584, 66), (12887, 523, 208), (66, 4786, 1610),
+         (4491, 66, 1637), (1175, 3280, 8), (818, 8, 2255), (4679, 823, 10), (71, 1291, 4321), (2645, 65, 1800), (16759, 662, 1041),
+         (19948, 1040, 560), (1092, 3354, 3601)]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', FORMS)
+def test_tile_forms(M, K, N, dtype):
+    args = _case(M, K, N, dtype, seed=M)
+    _check(_run(*args, 'elu'), *_oracle(*args, 'elu'))
+
+
 @gpu
 @pytest.mark.parametrize('dtype', [F32, BF16])
 def test_strides_offsets_and_leading_dimensions(dtype):

@@ -140,11 +140,12 @@ struct LinTile {
   static constexpr int NCH = BO * CK / NT;              // chunks a thread stages
   static constexpr int CPR = MC ? BO / X::VE : CK;      // chunks of a row in LDS
   static constexpr int READS = !MC ? 1 : sizeof(T) == 2 ? 2 : 4;   // LDS instructions of a fragment
-  static_assert(BO * CK % NT == 0, "whole chunks a thread");
+  static_assert(BO * CK % NT == 0 && (!MC || CPR == 8 || CPR % 16 == 0), "whole chunks a thread, exchanged within a row");
 
   static __device__ __forceinline__ int turn(int row) {            // what a row's chunk numbers are exchanged by
     if constexpr (!MC) return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
-    return sizeof(T) == 2 ? (row & 3) << 2 : 0;
+    if constexpr (sizeof(T) != 2) return 0;
+    return CPR == 8 ? (row & 2) << 1 : (row & 3) << 2;
   }
   static __device__ __forceinline__ int at(int row, int c) {       // byte offset of a chunk
     return row * (CPR * 16) + ((c ^ turn(row)) << 4);
@@ -749,25 +750,33 @@ struct LinPlan {
   int tm, tn, splits;
 };
 
-// How often the contraction of a product of 128 x 128 tiles is split: the cheapest of splits that fill one, two or three
-// blocks a CU, of a few small ones and of none.  A block's 128 bytes of contraction take `lat` microseconds where it is
-// alone on its CU and `thr` of the CU's time where it is not (both measured: fp32, bound by the matrix cores, 1.9 and 1.8;
-// bf16 0.55 and 0.47, 0.15 and 0.03 more for each operand that is read across; staged through registers 0.85 more, and 0.6
-// for each read across); a round starts and stores in 3, a second launch takes 6 and the partial sums their bytes at 8 TB/s
-// (from cache).  1472 x 512 x 768 bf16: 8.9 us unsplit, 13.3 in two; 2000 x 512 x 512 fp32: 24 in four, 27 in two.
-template <typename T, bool XMC, bool WMC>
-static LinPlan lin_plan(int M, int N, int K, int resident, bool aligned) {
+// How often the contraction of a product of TILE x TILE tiles is split, and what it then costs in microseconds: the cheapest
+// of splits that fill one to `resident` blocks a CU, of a few small ones and of none.  A block's 128 bytes of contraction
+// take `lat` where it is alone on its CU and `thr` of the CU's time where it is not; a round starts and stores in 3, a second
+// launch takes 6 and the partial sums their bytes at 8 TB/s (from cache).  Measured on operands that another kernel has just
+// written (not in this XCD's L2), 128 x 128: fp32, bound by the matrix cores, 1.9 and 1.8; bf16 0.6 and 0.47, 0.25 and 0.03
+// more for each operand that is read across; staged through registers 0.8 more, and 0.6 for each read across.  64 x 64: fp32
+// 0.53 and 0.48; bf16 0.25 and 0.2, 0.4 with an operand read across; through registers 0.5 more, and 0.3.  Forward, small and
+// large tiles: 1472 x 512 x 768 bf16 6.2 and 9.5 us, 512 x 1024 x 1024 6.8 and 13.3, 2000 x 512 x 512 fp32 13.3 and 23.7, but
+// 2048^3 bf16 30 and 25.5.
+template <typename T, bool XMC, bool WMC, int TILE>
+static LinPlan lin_plan(int M, int N, int K, int resident, bool aligned, bool split, double& best) {
+  static_assert(TILE == 64 || TILE == 128, "measured tiles");
   constexpr int BK = 128 / (int)sizeof(T), ACROSS = (int)XMC + (int)WMC;
-  const double lat = (sizeof(T) == 4 ? 1.9 : 0.55 + 0.15 * ACROSS) + (aligned ? 0.0 : 0.85 + 0.6 * ACROSS);
-  const double thr = sizeof(T) == 4 ? 1.8 : 0.47 + 0.03 * ACROSS;
-  LinPlan p{(M + 127) / 128, (N + 127) / 128, 1};
+  constexpr bool SMALL = TILE == 64, WIDE = sizeof(T) == 4;
+  const double lat = WIDE    ? (SMALL ? 0.53 : 1.9)
+                     : SMALL ? (ACROSS ? 0.4 : 0.25) + (aligned ? 0.0 : 0.5 + 0.3 * ACROSS)
+                             : 0.6 + 0.25 * ACROSS + (aligned ? 0.0 : 0.8 + 0.6 * ACROSS);
+  const double thr = WIDE ? (SMALL ? 0.48 : 1.8) : SMALL ? 0.2 + 0.04 * ACROSS + (aligned ? 0.0 : 0.1) : 0.47 + 0.03 * ACROSS;
+  LinPlan p{(M + TILE - 1) / TILE, (N + TILE - 1) / TILE, 1};
   const long long tiles = (long long)p.tm * p.tn, kt = (K + BK - 1) / BK;
   auto cost = [&](long long s) {
     const long long a_cu = (tiles * s + LIN_CUS - 1) / LIN_CUS, rounds = (a_cu + resident - 1) / resident;
     const double step = std::max(lat * (double)rounds, thr * (double)a_cu);
     return (double)((kt + s - 1) / s) * step + 3.0 * (double)rounds + (s > 1 ? 6.0 + (double)s * M * N * 8 / 8e6 : 0.0);
   };
-  double best = cost(1);
+  best = cost(1);
+  if (!split) return p;
   auto offer = [&](long long s) {
     if (s < 2 || s > kt || tiles * s > (long long)LIN_CUS * resident) return;
     const double c = cost(s);
@@ -860,7 +869,7 @@ static bool lin_flat(int M, int N) {
   return full > 1 && half * 11 <= full * 20;
 }
 
-enum LinForm { LIN_F_BIG, LIN_F_FLAT, LIN_F_SHORT, LIN_F_LONG };
+enum LinForm { LIN_F_BIG, LIN_F_FLAT, LIN_F_SHORT, LIN_F_LONG, LIN_F_SMALL };
 struct LinChoice {
   LinForm form;
   LinPlan plan;
@@ -869,8 +878,13 @@ template <typename T, bool XMC, bool WMC>
 static LinChoice lin_choose(int M, int N, int K, bool aligned) {
   if (aligned && lin_big<T>(M, N, K)) return {LIN_F_BIG, LinPlan{(M + 255) / 256, (N + 255) / 256, 1}};
   if (aligned && lin_flat<T>(M, N)) return {LIN_F_FLAT, LinPlan{(M + 63) / 64, (N + 127) / 128, 1}};
-  if (lin_short<XMC>(K)) return {LIN_F_SHORT, lin_plan<T, XMC, WMC>(M, N, K, 3, aligned)};
-  return {LIN_F_LONG, lin_plan<T, XMC, WMC>(M, N, K, 2, aligned)};
+  constexpr int SMALL_RESIDENT = 3;                        // of three 16 KB slots each (two slots, four blocks: 1000 x 2048 x 1000 17.8 us, 11.3)
+  double small_us, us;
+  const LinPlan small = lin_plan<T, XMC, WMC, 64>(M, N, K, SMALL_RESIDENT, aligned, true, small_us);
+  const bool brief = lin_short<XMC>(K);
+  const LinPlan large = lin_plan<T, XMC, WMC, 128>(M, N, K, brief ? 3 : 2, aligned, !brief, us);      // (a short contraction is split in small tiles)
+  if (small_us < us) return {LIN_F_SMALL, small};
+  return {brief ? LIN_F_SHORT : LIN_F_LONG, large};
 }
 
 template <typename T, bool XMC, bool WMC, bool ASYNC>
@@ -882,8 +896,9 @@ static int lin_sized(const LinOp<T>& x, const LinOp<T>& w, const LinEpi<T>& ep, 
     if constexpr (sizeof(T) == 4)
       if (c.form == LIN_F_FLAT) return lin_launch<T, XMC, WMC, 64, 128, 2, 2, 3, 128, 2, ASYNC, false>(x, w, ep, c.plan, part, s);
   }
+  if (c.form == LIN_F_SMALL) return lin_launch<T, XMC, WMC, 64, 64, 2, 2, 3, 128, 3, ASYNC, true>(x, w, ep, c.plan, part, s);
   if constexpr (!XMC)
-    if (c.form == LIN_F_SHORT) return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 3, 64, 3, ASYNC, true>(x, w, ep, c.plan, part, s);
+    if (c.form == LIN_F_SHORT) return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 3, 64, 3, ASYNC, false>(x, w, ep, c.plan, part, s);
   return lin_launch<T, XMC, WMC, 128, 128, 2, 2, 2, 128, 2, ASYNC, true>(x, w, ep, c.plan, part, s);
 }
 
@@ -923,7 +938,9 @@ struct LinBwdPlan {
 };
 template <typename T>
 static LinBwdPlan lin_bwd_plan(const vfd_linear_desc* d, const void* g, const void* w, const void* x, bool dx, bool dw) {
-  auto pitch = [](long long n) { return (n + 7) / 8 * 8; };
+  // whole cache lines where that adds at most a sixteenth (12 345 x 1001 x 1367: 62.8 and 81.0 us, 66.4 and 85.2 without;
+  // 60 001 x 333 x 777, where it would add a sixth: 104 and 131 us, 108 and 120 without)
+  auto pitch = [](long long n) { return (n + 63) / 64 * 64 * 16 <= n * 17 ? (n + 63) / 64 * 64 : (n + 7) / 8 * 8; };
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   LinBwdPlan p;
   // a product of few terms is not worth copies of its operands (1471 x 517 x 771: 47 us with and without)
@@ -950,7 +967,7 @@ static int lin_check(const char* what, const vfd_linear_desc* d) {
   VFD_REQUIRE(d && d->rows >= 0 && d->k >= 1 && d->n >= 1 && d->rows <= VFD_LINEAR_MAX && d->k <= VFD_LINEAR_MAX &&
                   d->n <= VFD_LINEAR_MAX && d->ldx >= d->k && d->act >= 0 && d->act < LIN_ACTS && (d->dtype == 0 || d->dtype == 1),
               "%s: bad descriptor", what);
-  const long long T = 128;
+  const long long T = 128;                                 // (a launch holds under 2^32 threads)
   VFD_REQUIRE(((long long)d->rows / T + 1) * (d->n / T + 1) < (1 << 24) && ((long long)d->rows / T + 1) * (d->k / T + 1) < (1 << 24) &&
                   ((long long)d->n / T + 1) * (d->k / T + 1) < (1 << 24),
               "%s: too many tiles", what);
