@@ -375,6 +375,15 @@ def test_very_wide_output():
 
 
 @gpu
+def test_most_rows():
+    from vfdepth_amd import kernels as KN
+    x = torch.empty(1 << 30, 1, device='cuda', dtype=BF16).uniform_(-2, 2)
+    w = torch.full((1, 1), 1.75, device='cuda', dtype=BF16)
+    y = KN.LinearAct.infer(x, w, None, None, 'none')
+    assert torch.equal(y, (x.float() * 1.75).bfloat16())
+
+
+@gpu
 def test_refusals():
     from vfdepth_amd import kernels as KN
     x, w, b, r, _ = _case(4, 8, 6, F32)

@@ -883,7 +883,7 @@ static LinChoice lin_choose(int M, int N, int K, bool aligned) {
   const LinPlan small = lin_plan<T, XMC, WMC, 64>(M, N, K, SMALL_RESIDENT, aligned, true, small_us);
   const bool brief = lin_short<XMC>(K);
   const LinPlan large = lin_plan<T, XMC, WMC, 128>(M, N, K, brief ? 3 : 2, aligned, !brief, us);      // (a short contraction is split in small tiles)
-  if (small_us < us) return {LIN_F_SMALL, small};
+  if (small_us < us && (long long)small.tm * small.tn < (1 << 24)) return {LIN_F_SMALL, small};
   return {brief ? LIN_F_SHORT : LIN_F_LONG, large};
 }
 
