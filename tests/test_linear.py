@@ -128,9 +128,9 @@ def test_c_refuses_null_tensors_and_small_workspaces():
     need = lib.vfd_linear_bwd_workspace(ctypes.byref(d), p, p, p, 1, 1)
     assert need > 0 and bwd(n=need - 1) == -1 and b'workspace' in lib.vfd_last_error()
     assert lib.vfd_linear_bwd_workspace(ctypes.byref(d), p, p, p, 0, 0) < need
-    odd = _desc(rows=50000, k=333, n=77, ldx=333, dtype=1)                       # rows of an odd length are laid out anew
-    even = _desc(rows=50000, k=334, n=78, ldx=334, dtype=1)
-    copies = 2 * (50000 * 80 + 77 * 336 + 50000 * 336)
+    odd = _desc(rows=50000, k=333, n=97, ldx=333, dtype=1)                       # rows of an odd length are laid out anew
+    even = _desc(rows=50000, k=334, n=98, ldx=334, dtype=1)
+    copies = 2 * (50000 * 104 + 97 * 336 + 50000 * 336)
     ws = [lib.vfd_linear_bwd_workspace(ctypes.byref(t), p, p, p, 1, 1) for t in (odd, even)]
     assert ws[0] >= copies and ws[1] < copies
     assert lib.vfd_linear_bwd_workspace(ctypes.byref(even), p, p, p + 2, 1, 1) >= ws[1] + 2 * 50000 * 336     # an odd start

@@ -728,7 +728,7 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
 }
 
 // Rows of an odd pitch or start laid out at a pitch of 16 bytes: read across (the gradients' products), 2-byte rows take 2.5
-// times as long through registers (12 345 x 1001 x 1367 bf16, data and weight gradient 263 us, 131 with this).
+// times as long through registers (12 345 x 1001 x 1367 bf16, data and weight gradient 328 us, 145 with this).
 template <typename T>
 __global__ __launch_bounds__(256) void lin_pack_k(const T* __restrict__ src, long long lds, T* __restrict__ dst, long long ldd,
                                                   int rows, int cols) {
@@ -945,8 +945,9 @@ static LinBwdPlan lin_bwd_plan(const vfd_linear_desc* d, const void* g, const vo
   auto pitch = [](long long n) { return (n + 63) / 64 * 64 * 16 <= n * 17 ? (n + 63) / 64 * 64 : (n + 7) / 8 * 8; };
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   LinBwdPlan p;
-  // a product of few terms is not worth copies of its operands (1471 x 517 x 771: 47 us with and without)
-  const bool pack = (dx || dw) && (double)d->rows * d->k * d->n > 1e9;
+  // a product of few terms is not worth copies of its operands (both gradients, with and without: 20 001 x 255 x 257 60 and
+  // 50 us, 2000 x 1001 x 1003 51 and 58)
+  const bool pack = (dx || dw) && (double)d->rows * d->k * d->n > 1.5e9;
   const bool bad_g = pack && !lin_dwords((const T*)g, d->n);
   p.gz = d->act != LIN_NONE || bad_g;
   p.w = pack && dx && !lin_dwords((const T*)w, d->k);
