@@ -317,6 +317,14 @@ def test_offsets_beyond_32_bits():
 
 
 @gpu
+def test_widest_rows_backward():
+    """2^25 columns and some: the weight's and bias's sums are over more columns than one launch has blocks of them for."""
+    x, w, b, g = (t.cuda() for t in _case(2, (1 << 25) + 19, F32, seed=4))
+    y, grads = _run(x, w, b, g)
+    _check((y, *grads), *_oracle(x, w, b, g))
+
+
+@gpu
 def test_streams_and_captured_graph():
     from vfdepth_amd import kernels as KN
     x, w, b, g = (t.cuda() for t in _case(500, 200, F32, seed=9))

@@ -375,6 +375,23 @@ def test_very_wide_output():
 
 
 @gpu
+def test_very_wide_output_backward():
+    """As many bias gradients as one launch has no blocks for.  A sum of two bf16 values is rounded once to 32 bits and once
+    to its type, and their products are exact in 32 bits: K = 1 leaves one addition a weight."""
+    x, w, b, _, g = _case(2, 1, (1 << 26) + 133, BF16, residual=False, seed=6)
+    y, dx, dw, db, _ = _run(x, w, b, None, g, 'none')
+    x, w, b = x.detach().double(), w.detach().double(), b.detach().double()
+    near = lambda t, v, e: bool(((t.double() - v).abs() <= e + HALF[BF16] * (v.abs() + e) + TINY).all())  # noqa: E731
+    with torch.no_grad():
+        assert torch.equal(db, (g[0].float() + g[1].float()).bfloat16())
+        z = x @ w.t()
+        assert near(y, z + b, 10 * U * (z.abs() + b.abs()))
+        gd = g.double()
+        assert near(dw, gd.t() @ x, 10 * U * (gd.abs().t() @ x.abs()))
+        assert near(dx, gd @ w, (w.shape[0] + 8) * U * (gd.abs() @ w.abs()))
+
+
+@gpu
 def test_most_rows():
     from vfdepth_amd import kernels as KN
     x = torch.empty(1 << 30, 1, device='cuda', dtype=BF16).uniform_(-2, 2)

@@ -465,7 +465,7 @@ static int ln_bwd_run(const vfd_norm_desc* d, const void* g, const void* x, cons
     return fail_launch("layer_norm_bwd");
   });
   if (e != VFD_OK || !cols) return e;
-  col_sums_k<float><<<cdiv(2 * (size_t)d->cols, COLSUM_COLS), 1024, 0, s>>>(part, nb, 2 * d->cols, d->cols, dw, db);
+  col_sums_k<float><<<col_sums_grid(2 * (size_t)d->cols), 1024, 0, s>>>(part, nb, 2 * d->cols, d->cols, dw, db);
   return fail_launch("layer_norm_bwd columns");
 }
 

@@ -1015,7 +1015,7 @@ static int lin_bwd_run(const vfd_linear_desc* d, const T* g, const T* z, const T
       lin_act_bwd_k<T, act()><<<grid, 256, 0, s>>>(g, z, gz, p.ldg, db ? part : nullptr, d->rows, d->n);
       return 0;
     });
-    if (db) col_sums_k<T><<<cdiv(d->n, COLSUM_COLS), 1024, 0, s>>>(part, strips, d->n, d->n, db, nullptr);
+    if (db) col_sums_k<T><<<col_sums_grid(d->n), 1024, 0, s>>>(part, strips, d->n, d->n, db, nullptr);
     if (int e = fail_launch("linear_bwd activation")) return e;
     if (gz) g = gz;
   }

@@ -295,34 +295,42 @@ static inline void zero_async(void* p, size_t bytes, hipStream_t s) {
 
 // Column sums of partial rows [nb][n] in row order: columns 0 .. split - 1 into a, the others into b (either may be
 // null).  64 slices of the rows a column: with one thread a column, 1024 dependent rounds of latency were the whole time.
+// Blocks walk over the columns: a block for every 16 of them would be more threads than a launch holds (under 2^32) from
+// 2^26 columns on.
 constexpr int COLSUM_COLS = 16;
+inline unsigned col_sums_grid(size_t n) {
+  const size_t need = (n + COLSUM_COLS - 1) / COLSUM_COLS;
+  return (unsigned)(need < (1u << 20) ? need : (1u << 20));
+}
 template <typename O>
 __global__ __launch_bounds__(1024) void col_sums_k(const float* __restrict__ part, int nb, int n, int split,
                                                    O* __restrict__ a, O* __restrict__ b) {
   __shared__ float sm[64][COLSUM_COLS + 1];
   const int lc = threadIdx.x % COLSUM_COLS, sl = threadIdx.x / COLSUM_COLS;
-  const size_t c = (size_t)blockIdx.x * COLSUM_COLS + lc;
-  float s = 0.f;
-  if (c < (size_t)n) {
-    int k = sl;
-    for (; k + 192 < nb; k += 256) {
-      const float v0 = part[(size_t)k * n + c], v1 = part[(size_t)(k + 64) * n + c], v2 = part[(size_t)(k + 128) * n + c],
-                  v3 = part[(size_t)(k + 192) * n + c];
-      s += (v0 + v1) + (v2 + v3);
+  for (size_t c0 = (size_t)blockIdx.x * COLSUM_COLS; c0 < (size_t)n; c0 += (size_t)gridDim.x * COLSUM_COLS) {
+    const size_t c = c0 + lc;
+    float s = 0.f;
+    if (c < (size_t)n) {
+      int k = sl;
+      for (; k + 192 < nb; k += 256) {
+        const float v0 = part[(size_t)k * n + c], v1 = part[(size_t)(k + 64) * n + c], v2 = part[(size_t)(k + 128) * n + c],
+                    v3 = part[(size_t)(k + 192) * n + c];
+        s += (v0 + v1) + (v2 + v3);
+      }
+      for (; k < nb; k += 64) s += part[(size_t)k * n + c];
     }
-    for (; k < nb; k += 64) s += part[(size_t)k * n + c];
-  }
-  sm[sl][lc] = s;
-  __syncthreads();
-  for (int h = 32; h > 0; h >>= 1) {
-    if (sl < h) sm[sl][lc] += sm[sl + h][lc];
+    sm[sl][lc] = s;                                        // (its own place: read by others only before the last barrier)
     __syncthreads();
-  }
-  if (sl == 0 && c < (size_t)n) {
-    if (c < (size_t)split) {
-      if (a != nullptr) st1(a + c, sm[0][lc]);
-    } else if (b != nullptr) {
-      st1(b + (c - split), sm[0][lc]);
+    for (int h = 32; h > 0; h >>= 1) {
+      if (sl < h) sm[sl][lc] += sm[sl + h][lc];
+      __syncthreads();
+    }
+    if (sl == 0 && c < (size_t)n) {
+      if (c < (size_t)split) {
+        if (a != nullptr) st1(a + c, sm[0][lc]);
+      } else if (b != nullptr) {
+        st1(b + (c - split), sm[0][lc]);
+      }
     }
   }
 }
