@@ -93,6 +93,15 @@ def test_c_refuses_null_tensors_and_small_workspaces():
     assert lib.vfd_layer_norm_fwd(ctypes.byref(_lib.NormDesc(0, 64, 64, 1e-5, 0)), *[None] * 7) == 0       # no rows
 
 
+@pytest.mark.parametrize('cols,dtype', [(1, 0), (16, 0), (16, 1), (4096, 1), (9001, 0)])
+def test_workspace_of_the_most_rows(cols, dtype):
+    from vfdepth_amd import _lib
+    lib = _lib.load()
+    ws = [lib.vfd_layer_norm_bwd_workspace(ctypes.byref(_lib.NormDesc(rows, cols, cols, 1e-5, dtype)))
+          for rows in ((1 << 31) - 1, (1 << 31) - 65)]
+    assert ws[0] == ws[1] > 0
+
+
 def test_descriptor_layout(tmp_path):
     import os
     import subprocess
@@ -314,6 +323,24 @@ def test_offsets_beyond_32_bits():
         ys = KN.LayerNorm.apply(xs, w, b, EPS)
         ds, = torch.autograd.grad(ys, xs, g[part].clone())
         assert torch.equal(y[part], ys) and torch.equal(dx[part], ds)
+
+
+@gpu
+def test_most_rows():
+    """2^31 - 1 rows of two values: the first and the last ones are the same as on their own."""
+    from vfdepth_amd import kernels as KN
+    rows = (1 << 31) - 1
+    x = torch.empty(rows, 2, dtype=BF16, device='cuda').normal_()
+    g = torch.empty(rows, 2, dtype=BF16, device='cuda').normal_()
+    w, b = torch.randn(2, device='cuda'), torch.randn(2, device='cuda', requires_grad=True)
+    y = KN.LayerNorm.apply(x.requires_grad_(True), w, b, EPS)
+    dx, db = torch.autograd.grad(y, (x, b), g)
+    for part in (slice(0, 7), slice(rows - 131, rows)):
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys = KN.LayerNorm.apply(xs, w, b, EPS)
+        ds, = torch.autograd.grad(ys, xs, g[part].clone())
+        assert torch.equal(y[part], ys) and torch.equal(dx[part], ds)
+    assert db.shape == (2,) and bool(torch.isfinite(db).all())
 
 
 @gpu

@@ -415,7 +415,7 @@ constexpr int LN_FWD_GRID = 1024;
 // 28.4 with 512, 26.6 with 1024.
 static int ln_bwd_blocks(int rows, int rb, int w, int e) {
   const int most = w > 1 ? 512 : (e >= 16 ? 768 : 1024);
-  const int need = (rows + rb - 1) / rb;
+  const int need = (rows - 1) / rb + 1;                      // (rows up to 2^31 - 1: none added to them)
   return need < most ? need : most;
 }
 
@@ -438,7 +438,7 @@ static int ln_fwd_run(const vfd_norm_desc* d, const void* x, const float* w, con
       ln_fwd_wide_k<T><<<grid, LN_WIDE, 0, s>>>((const T*)x, d->ldx, w, b, (T*)y, mean, rstd, d->rows, d->cols, d->eps);
     } else {
       typedef LnGroup<T, l(), wv(), nv()> Gr;
-      const int need = (d->rows + Gr::RB - 1) / Gr::RB, grid = need < LN_FWD_GRID ? need : LN_FWD_GRID;
+      const int need = (d->rows - 1) / Gr::RB + 1, grid = need < LN_FWD_GRID ? need : LN_FWD_GRID;
       ln_fwd_k<T, l(), wv(), nv()><<<grid, Gr::BLOCK, 0, s>>>((const T*)x, d->ldx, w, b, (T*)y, mean, rstd, d->rows, d->cols, d->eps);
     }
     return fail_launch("layer_norm_fwd");
