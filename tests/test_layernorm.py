@@ -291,6 +291,17 @@ def test_refusals():
 
 
 @gpu
+def test_refuses_sizes_that_32_bits_do_not_hold():
+    from vfdepth_amd import kernels as KN
+    x = torch.randn(1, 1, device='cuda')
+    for C in ((1 << 28) + 1, (1 << 32) + 8):                 # (the second is 8 in 32 bits)
+        with pytest.raises(RuntimeError, match='2\\^28 at most'):
+            KN.LayerNorm.apply(x.expand(1, C), None, None, EPS)
+    with pytest.raises(RuntimeError, match='rows'):
+        KN.LayerNorm.apply(x.expand((1 << 31) + 3, 1), None, None, EPS)
+
+
+@gpu
 def test_module_parameters_in_bf16_and_autocast():
     from vfdepth_amd import layers
     ln = torch.nn.LayerNorm(96).cuda()

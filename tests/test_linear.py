@@ -420,6 +420,19 @@ def test_refusals():
 
 
 @gpu
+def test_refuses_sizes_that_32_bits_do_not_hold():
+    from vfdepth_amd import kernels as KN
+    one = torch.randn(1, 1, device='cuda')
+    for n in ((1 << 30) + 1, (1 << 32) + 8):                         # (the second is 8 in 32 bits)
+        with pytest.raises(RuntimeError, match='at most 2\\^30'):
+            KN.LinearAct.apply(one, one.expand(n, 1), None, None, 'none')
+        with pytest.raises(RuntimeError, match='at most 2\\^30'):
+            KN.LinearAct.apply(one.expand(1, n), one.expand(1, n), None, None, 'none')
+    with pytest.raises(RuntimeError, match='descriptor|rows'):
+        KN.LinearAct.apply(one.expand((1 << 31) + 3, 1), one, None, None, 'none')
+
+
+@gpu
 @pytest.mark.parametrize('fmt', [torch.channels_last, torch.contiguous_format])
 def test_conv_1x1(fmt):
     from vfdepth_amd import layers

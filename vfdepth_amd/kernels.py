@@ -2183,8 +2183,8 @@ class LayerNorm(torch.autograd.Function):
         lib = L.load()
         _check_device(x, 'layer norm input')
         C = x.shape[-1] if x.dim() else 0
-        if C == 0:
-            raise RuntimeError(f'layer norm: the last dimension must hold values, got {tuple(x.shape)}')
+        if not 0 < C <= 1 << 28:
+            raise RuntimeError(f'layer norm: the last dimension must hold values, 2^28 at most, got {tuple(x.shape)}')
         if weight is not None:
             weight = _param(weight, x, torch.float32, (C,), 'layer norm weight')
         if bias is not None:
@@ -2256,6 +2256,8 @@ class LinearAct(torch.autograd.Function):
             raise RuntimeError(f'linear: x [..., K] and weight [N, K], K and N at least 1, got {tuple(x.shape)} and '
                                f'{tuple(getattr(weight, "shape", ()))}')
         N, K = weight.shape
+        if N > 1 << 30 or K > 1 << 30:
+            raise RuntimeError(f'linear: K and N are at most 2^30, got weight {tuple(weight.shape)}')
         dtype, shape = x.dtype, (*x.shape[:-1], N)
         code = _dt(x)
         weight = _param(weight, x, dtype, (N, K), 'linear weight')
