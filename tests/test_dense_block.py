@@ -94,3 +94,78 @@ def test_block_step_captured():
         torch.cuda.synchronize()
         want_n, want = step()
         assert torch.equal(norm_, want_n) and all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+class Map(torch.nn.Module):
+    """The map forms: channel norm, 1x1 convolution with activation and residual."""
+
+    def __init__(self, width):
+        super().__init__()
+        self.norm, self.conv = torch.nn.LayerNorm(width), torch.nn.Conv2d(width, width, 1)
+
+    def forward(self, x):
+        from vfdepth_amd import layers
+        return layers.linear_act(self.conv, layers.channel_norm(self.norm, x), 'silu', x)
+
+
+def _plain_block(m, x):
+    f = torch.nn.functional
+    if isinstance(m, Block):
+        return m.down(f.gelu(m.up(m.norm(x)))) + x
+    return f.silu(m.conv(m.norm(x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2))) + x
+
+
+def _recorded_cases():
+    return [(Block(24, 40).cuda(), (5, 24)), (Map(16).cuda(), (2, 16, 3, 4))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('grad', [False, True])
+def test_traced_block(grad):
+    """A trace, with a graph or without, computes its outputs from its inputs as the block does."""
+    import warnings
+    for m, shape in _recorded_cases():
+        with torch.set_grad_enabled(grad), warnings.catch_warnings():
+            warnings.simplefilter('ignore', torch.jit.TracerWarning)
+            traced = torch.jit.trace(m, torch.randn(shape, device='cuda'), check_trace=False)
+            for _ in range(3):
+                x = torch.randn(shape, device='cuda')
+                junk = [torch.full(shape, float('nan'), device='cuda') for _ in range(8)]      # (for memory not written)
+                del junk
+                assert torch.allclose(traced(x), _plain_block(m, x), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_and_functional_transforms(grad):
+    """The tangent of a dual input is carried through, with a graph or without, and a transform sees the operators."""
+    import torch.autograd.forward_ad as fw
+    for m, shape in _recorded_cases():
+        x, v = torch.randn(shape, device='cuda'), torch.randn(shape, device='cuda')
+        with torch.set_grad_enabled(grad):
+            with fw.dual_level():
+                got = fw.unpack_dual(m(fw.make_dual(x, v)))
+                want = fw.unpack_dual(_plain_block(m, fw.make_dual(x, v)))
+                assert got.tangent is not None
+                assert all(torch.allclose(a, b, rtol=1e-5, atol=1e-5) for a, b in zip(got, want))
+            y, t = torch.func.jvp(m, (x,), (v,))
+            assert torch.allclose(y, want.primal, rtol=1e-5, atol=1e-5) and torch.allclose(t, want.tangent, rtol=1e-5, atol=1e-5)
+            xs = torch.stack([x, v])
+            assert torch.allclose(torch.func.vmap(m)(xs), torch.stack([_plain_block(m, a) for a in xs]), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_kernel_calls_refuse_forward_mode():
+    """The calls below the layers have no tangents to give: refused, with a graph or without."""
+    import torch.autograd.forward_ad as fw
+    from vfdepth_amd import kernels as KN
+    x, w = torch.randn(4, 8, device='cuda'), torch.randn(6, 8, device='cuda')
+    with torch.no_grad(), fw.dual_level():
+        dual = fw.make_dual(x, x)
+        for call in (lambda: KN.LayerNorm.infer(dual, None, None, 1e-5), lambda: KN.LayerNorm.apply(dual, None, None, 1e-5),
+                     lambda: KN.LinearAct.infer(dual, w, None, None, 'gelu'), lambda: KN.LinearAct.apply(dual, w, None, None, 'gelu')):
+            with pytest.raises(NotImplementedError, match='jvp'):
+                call()
+    traced = torch.jit.trace(lambda t: KN.LayerNorm.infer(t, None, None, 1e-5), x, check_trace=False)
+    z = torch.randn(4, 8, device='cuda')
+    assert torch.equal(traced(z), KN.LayerNorm.infer(z, None, None, 1e-5))

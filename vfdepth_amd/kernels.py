@@ -13,6 +13,7 @@ import weakref
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -2148,6 +2149,13 @@ def _once(fn):
     return staticmethod(backward)
 
 
+def seen_through():
+    """Whether something has to see a call as torch's operators: a tracer that records it (it would keep only the output's
+    allocation), a forward-mode level (the output would carry no tangent) or a functional transform."""
+    return (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+            or torch._C._are_functorch_transforms_active())
+
+
 def _param(t, x, dtype, shape, what):
     """A further operand of x's operator, dense: on x's device, of this type and shape."""
     if not torch.is_tensor(t) or t.get_device() != x.get_device():
@@ -2176,6 +2184,8 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     def infer(x, weight, bias, eps):
         """The forward without a graph: no statistics are kept."""
+        if seen_through():
+            return LayerNorm.apply(x, weight, bias, eps)
         return LayerNorm._run(x, weight, bias, eps, False)[0]
 
     @staticmethod
@@ -2244,6 +2254,8 @@ class LinearAct(torch.autograd.Function):
     @staticmethod
     def infer(x, weight, bias, residual, act):
         """The forward without a graph: no pre-activation is kept."""
+        if seen_through():
+            return LinearAct.apply(x, weight, bias, residual, act)
         return LinearAct._run(x, weight, bias, residual, act, False)[0]
 
     @staticmethod

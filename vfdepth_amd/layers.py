@@ -150,10 +150,10 @@ def max_pool_stem(pool, x):
 def layer_norm(ln, x):
     """nn.LayerNorm `ln` over the last dimension of x [..., C]: the HIP kernel pair (layernorm.hip) for fp32 or bf16
     activations on the GPU (parameters and statistics fp32, the output in x's type), the module otherwise (CPU, other
-    types, several normalised dimensions)."""
-    if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and len(ln.normalized_shape) == 1 and x.dim() >= 1
-            and x.shape[-1] == ln.normalized_shape[0]):
-        from . import kernels as KN
+    types, several normalised dimensions; under torch.jit.trace, forward-mode differentiation or a functional transform)."""
+    from . import kernels as KN
+    if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not KN.seen_through() and len(ln.normalized_shape) == 1
+            and x.dim() >= 1 and x.shape[-1] == ln.normalized_shape[0]):
         w, b = (p if p is None or p.dtype == torch.float32 else p.float() for p in (ln.weight, ln.bias))
         return (KN.LayerNorm.apply if torch.is_grad_enabled() else KN.LayerNorm.infer)(x, w, b, ln.eps)
     return ln(x)
@@ -172,20 +172,21 @@ _ACTS = {'none': lambda z: z, 'relu': F.relu, 'lrelu': lambda z: F.leaky_relu(z,
 def linear_act(lin, x, act='none', residual=None):
     """act(lin(x)) + residual for `lin` an nn.Linear (x [..., K]) or a 1x1 nn.Conv2d (x a map [N, K, H, W]): the product
     with bias, activation and residual in its epilogue (linear.hip) for fp32 or bf16 on the GPU, under autocast in its
-    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types).  act: 'none',
-    'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The convolution's output is channels-last; a channels-last map
-    is read where it lies, another one is copied into that layout first."""
+    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types; under
+    torch.jit.trace, forward-mode differentiation or a functional transform).  act: 'none', 'relu', 'lrelu' (slope 0.1),
+    'elu', 'gelu', 'silu'.  The kernel's output for a convolution is channels-last; a channels-last map is read where it
+    lies, another one is copied into that layout first."""
     if act not in _ACTS:
         raise ValueError(f'linear_act: act is one of {", ".join(_ACTS)}, got {act!r}')
     conv = isinstance(lin, nn.Conv2d)
     if conv and not (tuple(lin.kernel_size) == (1, 1) and tuple(lin.stride) == (1, 1) and lin.groups == 1
                      and lin.padding in (0, (0, 0), 'valid', 'same') and x.dim() == 4):
         raise ValueError('linear_act: a convolution is 1x1, of stride 1, without padding or groups, on a map [N, K, H, W]')
+    from . import kernels as KN
     dt = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else x.dtype
-    if not (x.is_cuda and dt in (torch.float32, torch.bfloat16)):
+    if not x.is_cuda or dt not in (torch.float32, torch.bfloat16) or KN.seen_through():
         y = _ACTS[act](lin(x))
         return y if residual is None else y + residual
-    from . import kernels as KN
     w, b = lin.weight, lin.bias
     if torch.is_autocast_enabled('cuda'):
         x, w, b, residual = (None if t is None else t.to(dt) for t in (x, w, b, residual))
