@@ -169,3 +169,94 @@ def test_kernel_calls_refuse_forward_mode():
     traced = torch.jit.trace(lambda t: KN.LayerNorm.infer(t, None, None, 1e-5), x, check_trace=False)
     z = torch.randn(4, 8, device='cuda')
     assert torch.equal(traced(z), KN.LayerNorm.infer(z, None, None, 1e-5))
+
+
+class _Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _Shifted(torch.nn.LayerNorm):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+def _hooked(kind):
+    """(module, whether it is a linear layer) with something hanging on its call."""
+    if kind == 'subclass':
+        return _Doubled(24, 16), True
+    if kind == 'norm_subclass':
+        return _Shifted(24), False
+    m = torch.nn.LayerNorm(24) if kind.startswith('norm') else torch.nn.Linear(24, 16)
+    if kind in ('pre', 'norm_pre'):
+        m.register_forward_pre_hook(lambda mod, args: (args[0] * 3,))
+    elif kind in ('post', 'norm_post'):
+        m.register_forward_hook(lambda mod, args, out: out - 2)
+    elif kind == 'backward':
+        m.register_full_backward_hook(lambda mod, gi, go: (gi[0] * 5,))
+    elif kind == 'instance':
+        m.forward = lambda x: torch.nn.functional.linear(x, m.weight)
+    elif kind == 'weight_norm':
+        m = torch.nn.utils.weight_norm(m)                     # the weight is computed by a hook before each call
+    elif kind == 'parametrized':
+        m = torch.nn.utils.parametrizations.weight_norm(m)
+    return m, not kind.startswith('norm')
+
+
+HOOKED = ['pre', 'post', 'backward', 'instance', 'subclass', 'weight_norm', 'parametrized', 'norm_pre', 'norm_post', 'norm_subclass']
+
+
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('grad', [True, False])
+@pytest.mark.parametrize('kind', HOOKED)
+def test_what_hangs_on_a_module(kind, grad, device):
+    """Hooks, forwards of subclasses and of objects, and weights computed before a call count on either device."""
+    from vfdepth_amd import layers
+    torch.manual_seed(3)
+    m, linear_ = _hooked(kind)
+    m = m.to(device)
+    with torch.no_grad():
+        for p in m.parameters():                              # a weight that was computed at construction is out of date now
+            p.mul_(1.5)
+    x = torch.randn(7, 24, device=device, requires_grad=grad)
+    run = (lambda: layers.linear_act(m, x, 'silu')) if linear_ else (lambda: layers.layer_norm(m, x))
+    plain = (lambda: torch.nn.functional.silu(m(x))) if linear_ else (lambda: m(x))
+    with torch.set_grad_enabled(grad):
+        y, want = run(), plain()
+        assert torch.allclose(y, want, rtol=1e-5, atol=1e-5)
+        if grad:
+            ps = [x] + list(m.parameters())
+            for a, b in zip(*(torch.autograd.grad(t.square().sum(), ps, allow_unused=True) for t in (y, want))):
+                assert (a is None) == (b is None) and (a is None or torch.allclose(a, b, rtol=1e-4, atol=1e-4))
+
+
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_global_hooks_see_the_modules(device):
+    from vfdepth_amd import layers
+    ln, lin = torch.nn.LayerNorm(8).to(device), torch.nn.Linear(8, 8).to(device)
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: seen.append(mod))
+    try:
+        layers.linear_act(lin, layers.layer_norm(ln, torch.randn(3, 8, device=device)), 'relu')
+    finally:
+        handle.remove()
+    assert seen == [ln, lin]
+
+
+@pytest.mark.gpu
+def test_plain_modules_take_the_kernels():
+    """Ordinary modules, a subclass without a forward and a parametrized weight are not sent to the module."""
+    from vfdepth_amd import layers
+
+    class Named(torch.nn.Linear):
+        pass
+    para = torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(24, 16))
+    for m in (torch.nn.Linear(24, 16), Named(24, 16), para, torch.nn.Conv2d(24, 16, 1), layers.conv2d_block(24, 16, 1)[0]):
+        m = m.cuda()
+        x = torch.randn(2, 24, 3, 5, device='cuda') if isinstance(m, torch.nn.Conv2d) else torch.randn(7, 24, device='cuda')
+        fn = layers.linear_act(m, x, 'silu').grad_fn
+        while 'Permute' in type(fn).__name__:
+            fn = fn.next_functions[0][0]
+        assert type(fn).__name__ == 'LinearActBackward'
+    y = layers.layer_norm(torch.nn.LayerNorm(8).cuda(), torch.randn(3, 8, device='cuda'))
+    assert type(y.grad_fn).__name__ == 'LayerNormBackward'

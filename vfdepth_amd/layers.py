@@ -147,13 +147,26 @@ def max_pool_stem(pool, x):
     return pool(x)
 
 
+_FORWARDS = {nn.LayerNorm.forward, nn.Linear.forward, nn.Conv2d.forward}
+
+
+def _only_forward(m):
+    """Whether calling module `m` is its class's forward and nothing else, so that a kernel may take its parameters
+    instead: no hooks (weight normalisation computes the weight in one), no forward of a subclass or of the object."""
+    return (type(m).forward in _FORWARDS
+            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks
+                     or 'forward' in m.__dict__ or torch.nn.modules.module._has_any_global_hook())
+            and getattr(type(m), '_conv_forward', None) in (None, nn.Conv2d._conv_forward, ReflectConv2d._conv_forward))
+
+
 def layer_norm(ln, x):
     """nn.LayerNorm `ln` over the last dimension of x [..., C]: the HIP kernel pair (layernorm.hip) for fp32 or bf16
     activations on the GPU (parameters and statistics fp32, the output in x's type), the module otherwise (CPU, other
-    types, several normalised dimensions; under torch.jit.trace, forward-mode differentiation or a functional transform)."""
+    types, several normalised dimensions; a module with hooks or a forward of its own; under torch.jit.trace, forward-mode
+    differentiation or a functional transform)."""
     from . import kernels as KN
-    if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not KN.seen_through() and len(ln.normalized_shape) == 1
-            and x.dim() >= 1 and x.shape[-1] == ln.normalized_shape[0]):
+    if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not KN.seen_through() and _only_forward(ln)
+            and len(ln.normalized_shape) == 1 and x.dim() >= 1 and x.shape[-1] == ln.normalized_shape[0]):
         w, b = (p if p is None or p.dtype == torch.float32 else p.float() for p in (ln.weight, ln.bias))
         return (KN.LayerNorm.apply if torch.is_grad_enabled() else KN.LayerNorm.infer)(x, w, b, ln.eps)
     return ln(x)
@@ -172,10 +185,10 @@ _ACTS = {'none': lambda z: z, 'relu': F.relu, 'lrelu': lambda z: F.leaky_relu(z,
 def linear_act(lin, x, act='none', residual=None):
     """act(lin(x)) + residual for `lin` an nn.Linear (x [..., K]) or a 1x1 nn.Conv2d (x a map [N, K, H, W]): the product
     with bias, activation and residual in its epilogue (linear.hip) for fp32 or bf16 on the GPU, under autocast in its
-    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types; under
-    torch.jit.trace, forward-mode differentiation or a functional transform).  act: 'none', 'relu', 'lrelu' (slope 0.1),
-    'elu', 'gelu', 'silu'.  The kernel's output for a convolution is channels-last; a channels-last map is read where it
-    lies, another one is copied into that layout first."""
+    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types; a
+    module with hooks or a forward of its own; under torch.jit.trace, forward-mode differentiation or a functional
+    transform).  act: 'none', 'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The kernel's output for a convolution
+    is channels-last; a channels-last map is read where it lies, another one is copied into that layout first."""
     if act not in _ACTS:
         raise ValueError(f'linear_act: act is one of {", ".join(_ACTS)}, got {act!r}')
     conv = isinstance(lin, nn.Conv2d)
@@ -184,7 +197,7 @@ def linear_act(lin, x, act='none', residual=None):
         raise ValueError('linear_act: a convolution is 1x1, of stride 1, without padding or groups, on a map [N, K, H, W]')
     from . import kernels as KN
     dt = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else x.dtype
-    if not x.is_cuda or dt not in (torch.float32, torch.bfloat16) or KN.seen_through():
+    if not x.is_cuda or dt not in (torch.float32, torch.bfloat16) or KN.seen_through() or not _only_forward(lin):
         y = _ACTS[act](lin(x))
         return y if residual is None else y + residual
     w, b = lin.weight, lin.bias
