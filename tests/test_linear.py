@@ -464,6 +464,34 @@ def test_autocast():
 
 
 @gpu
+@pytest.mark.parametrize('conv', [False, True])
+def test_autocast_adds_a_wider_residual_in_its_type(conv):
+    """Under bf16 autocast an fp32 residual stays fp32 and makes the output fp32, as in torch: only the product and its
+    activation are rounded to bf16, and the residual's gradient is the incoming one."""
+    from vfdepth_amd import layers
+    lin = (torch.nn.Conv2d(64, 72, 1) if conv else torch.nn.Linear(64, 72)).cuda()
+    x, _, _, _, _ = _case(90, 64, 72, BF16, seed=14)
+    gen = torch.Generator().manual_seed(15)
+    r, g = (torch.randn(90, 72, generator=gen).cuda() for _ in range(2))
+    shaped = (lambda t: t.view(2, 5, 9, -1).permute(0, 3, 1, 2)) if conv else (lambda t: t)
+    flat = (lambda t: t.permute(0, 2, 3, 1).reshape(90, -1)) if conv else (lambda t: t)
+    x.requires_grad_(True), r.requires_grad_(True)
+    for grad in (True, False):
+        with torch.autocast('cuda', dtype=BF16), torch.set_grad_enabled(grad):
+            y = layers.linear_act(lin, shaped(x), 'gelu', shaped(r))
+            assert y.dtype == (_slope(lin(shaped(x)).detach(), 'none')[0] + shaped(r)).dtype == F32
+        w, b = lin.weight.detach().view(72, 64).to(BF16), lin.bias.detach().to(BF16)
+        vals, tol = _oracle(x, w, b, None, g.to(BF16), 'gelu')
+        yd, rd = flat(y).detach().cpu().double(), r.detach().cpu().double()
+        lim = tol[0] + HALF[BF16] * (vals[0].abs() + tol[0]) + U * (yd.abs() + rd.abs())
+        assert bool(((yd - rd - vals[0]).abs() <= lim).all())
+        if grad:
+            dx, dw, db, dr = torch.autograd.grad(y, (x, lin.weight, lin.bias, r), shaped(g))
+            assert torch.equal(dr, g)
+            _check([None, dx, dw.view(72, 64).to(BF16), db.to(BF16)], vals, tol)
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """Input, output and weight-gradient reads of 2.2 billion values each: rows at both ends against the oracle."""
     from vfdepth_amd import kernels as KN

@@ -185,10 +185,11 @@ _ACTS = {'none': lambda z: z, 'relu': F.relu, 'lrelu': lambda z: F.leaky_relu(z,
 def linear_act(lin, x, act='none', residual=None):
     """act(lin(x)) + residual for `lin` an nn.Linear (x [..., K]) or a 1x1 nn.Conv2d (x a map [N, K, H, W]): the product
     with bias, activation and residual in its epilogue (linear.hip) for fp32 or bf16 on the GPU, under autocast in its
-    type (then also the residual's and the output's); the module + torch ops otherwise (CPU, other types; a
-    module with hooks or a forward of its own; under torch.jit.trace, forward-mode differentiation or a functional
-    transform).  act: 'none', 'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The kernel's output for a convolution
-    is channels-last; a channels-last map is read where it lies, another one is copied into that layout first."""
+    type (a residual of another type is then added by torch, in the wider of the two); the module + torch ops otherwise
+    (CPU, other types; a module with hooks or a forward of its own; under torch.jit.trace, forward-mode differentiation
+    or a functional transform).  act: 'none', 'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The kernel's output for
+    a convolution is channels-last; a channels-last map is read where it lies, another one is copied into that layout
+    first."""
     if act not in _ACTS:
         raise ValueError(f'linear_act: act is one of {", ".join(_ACTS)}, got {act!r}')
     conv = isinstance(lin, nn.Conv2d)
@@ -196,18 +197,23 @@ def linear_act(lin, x, act='none', residual=None):
                      and lin.padding in (0, (0, 0), 'valid', 'same') and x.dim() == 4):
         raise ValueError('linear_act: a convolution is 1x1, of stride 1, without padding or groups, on a map [N, K, H, W]')
     from . import kernels as KN
-    dt = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else x.dtype
+    amp = torch.is_autocast_enabled('cuda')
+    dt = torch.get_autocast_dtype('cuda') if amp else x.dtype
     if not x.is_cuda or dt not in (torch.float32, torch.bfloat16) or KN.seen_through() or not _only_forward(lin):
         y = _ACTS[act](lin(x))
         return y if residual is None else y + residual
-    w, b = lin.weight, lin.bias
-    if torch.is_autocast_enabled('cuda'):
-        x, w, b, residual = (None if t is None else t.to(dt) for t in (x, w, b, residual))
+    w, b, late = lin.weight, lin.bias, None
+    if amp:
+        x, w, b = (None if t is None else t.to(dt) for t in (x, w, b))
+        if residual is not None and residual.dtype != dt:    # a wider stream stays as wide as it is: torch's addition
+            residual, late = None, residual
     run = KN.LinearAct.apply if torch.is_grad_enabled() else KN.LinearAct.infer
     if not conv:
-        return run(x, w, b, residual, act)
-    r = residual.permute(0, 2, 3, 1) if residual is not None else None
-    return run(x.permute(0, 2, 3, 1), w.flatten(1), b, r, act).permute(0, 3, 1, 2)
+        y = run(x, w, b, residual, act)
+    else:
+        r = residual.permute(0, 2, 3, 1) if residual is not None else None
+        y = run(x.permute(0, 2, 3, 1), w.flatten(1), b, r, act).permute(0, 3, 1, 2)
+    return y if late is None else y + late
 
 
 class BasicBlock(nn.Module):
