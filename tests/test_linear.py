@@ -464,6 +464,23 @@ def test_autocast():
 
 
 @gpu
+def test_autocast_leaves_64_bits():
+    """As torch's autocast: fp64 operands are not cast, and mixed ones do not pass."""
+    from vfdepth_amd import layers
+    lin = torch.nn.Linear(24, 16).cuda().double()
+    x = torch.randn(7, 24, device='cuda', dtype=torch.float64, requires_grad=True)
+    with torch.autocast('cuda', dtype=BF16):
+        y, want = layers.linear_act(lin, x, 'elu', x[:, :16]), torch.nn.functional.elu(lin(x)) + x[:, :16]
+        assert y.dtype == torch.float64 and torch.allclose(y, want, rtol=1e-12, atol=1e-12)
+        assert torch.autograd.grad(y.sum(), x)[0].dtype == torch.float64
+        narrow = torch.nn.Linear(24, 16).cuda()
+        for m, t in ((lin, x.detach().float()), (narrow, torch.ones(7, 24, dtype=torch.int64, device='cuda'))):
+            for call in (lambda: m(t), lambda: layers.linear_act(m, t, 'elu')):
+                with pytest.raises(RuntimeError):
+                    call()
+
+
+@gpu
 @pytest.mark.parametrize('conv', [False, True])
 def test_autocast_adds_a_wider_residual_in_its_type(conv):
     """Under bf16 autocast an fp32 residual stays fp32 and makes the output fp32, as in torch: only the product and its

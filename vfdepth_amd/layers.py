@@ -178,6 +178,7 @@ def channel_norm(ln, x):
     return layer_norm(ln, x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
 
 
+_CAST = (torch.float32, torch.bfloat16, torch.float16)
 _ACTS = {'none': lambda z: z, 'relu': F.relu, 'lrelu': lambda z: F.leaky_relu(z, 0.1), 'elu': F.elu, 'gelu': F.gelu,
          'silu': F.silu}
 
@@ -198,13 +199,14 @@ def linear_act(lin, x, act='none', residual=None):
         raise ValueError('linear_act: a convolution is 1x1, of stride 1, without padding or groups, on a map [N, K, H, W]')
     from . import kernels as KN
     amp = torch.is_autocast_enabled('cuda')
-    dt = torch.get_autocast_dtype('cuda') if amp else x.dtype
+    # (autocast casts floats of up to 32 bits, and leaves what is wider, or whole numbers, to the module)
+    dt = torch.get_autocast_dtype('cuda') if amp and x.dtype in _CAST else x.dtype
     if not x.is_cuda or dt not in (torch.float32, torch.bfloat16) or KN.seen_through() or not _only_forward(lin):
         y = _ACTS[act](lin(x))
         return y if residual is None else y + residual
     w, b, late = lin.weight, lin.bias, None
     if amp:
-        x, w, b = (None if t is None else t.to(dt) for t in (x, w, b))
+        x, w, b = (t.to(dt) if t is not None and t.dtype in _CAST else t for t in (x, w, b))
         if residual is not None and residual.dtype != dt:    # a wider stream stays as wide as it is: torch's addition
             residual, late = None, residual
     run = KN.LinearAct.apply if torch.is_grad_enabled() else KN.LinearAct.infer
