@@ -140,6 +140,17 @@ def test_c_refuses_null_tensors_and_small_workspaces():
     assert lib.vfd_linear_fwd(ctypes.byref(_desc(rows=0)), *[no] * 7, 0, no) == 0
 
 
+@pytest.mark.parametrize('dtype', [0, 1])
+def test_bias_gradient_alone_needs_no_activation_gradient(dtype):
+    """Only column sums: one fp32 row for each of at most 1024 row blocks."""
+    from vfdepth_amd import _lib
+    lib = _lib.load()
+    for act in (0, 3, 4):
+        d = _desc(rows=92160, k=256, n=1024, act=act, ldx=256, dtype=dtype)
+        need = lib.vfd_linear_bwd_workspace(ctypes.byref(d), 1 << 40, 1 << 40, 1 << 40, 0, 0)
+        assert 0 < need <= 1024 * 1024 * 4, need
+
+
 def test_descriptor_layout(tmp_path):
     import os
     import subprocess
@@ -297,6 +308,19 @@ def test_parts_of_the_gradient(act):
         y = KN.LinearAct.apply(*leaves, act)
         grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], g))
         _check([y] + [next(grads) if n else None for n in need], vals, tol)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('act', ACTS)
+def test_bias_gradient_alone(act, dtype):
+    """No product reads the activation's gradient here: the sums are the same bits as beside the other gradients."""
+    from vfdepth_amd import kernels as KN
+    x, w, b, _, g = _case(2100, 96, 300, dtype, seed=21)
+    want = _run(x, w, b, None, g, act)[3]
+    b = b.detach().requires_grad_(True)
+    db, = torch.autograd.grad(KN.LinearAct.apply(x.detach(), w.detach(), b, None, act), b, g)
+    assert torch.equal(db, want)
 
 
 @gpu

@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256) void lin_act_bwd_k(const T* __restrict__ g, co
           s[j] += f[u][j];
           o[j] = (T)f[u][j];
         }
-        if (ACT == LIN_NONE && gz == nullptr) continue;
+        if (gz == nullptr) continue;                       // only the sums are wanted
         const size_t at = (size_t)(m0 + u * step) * ldg + n;
         if (cnt == V) {
           *reinterpret_cast<vec*>(gz + at) = o;
@@ -931,7 +931,7 @@ static size_t lin_fwd_ws(const vfd_linear_desc* d) {
   return lin_is_thin(d) ? 0 : lin_part_bytes<T, false, false>(d->rows, d->n, d->k);
 }
 
-// The backward's workspace: gz (where an activation makes one, or g cannot be streamed), copies of W and x where those
+// The backward's workspace: gz (where an activation makes one for a product, or g cannot be streamed), copies of W and x where those
 // cannot, and one scratch for the steps' partial sums, which follow each other on one stream.
 struct LinBwdPlan {
   long long ldg, ldw, ldx;       // pitches of the operands that the products read
@@ -949,7 +949,7 @@ static LinBwdPlan lin_bwd_plan(const vfd_linear_desc* d, const void* g, const vo
   // 50 us, 2000 x 1001 x 1003 51 and 58)
   const bool pack = (dx || dw) && (double)d->rows * d->k * d->n > 1.5e9;
   const bool bad_g = pack && !lin_dwords((const T*)g, d->n);
-  p.gz = d->act != LIN_NONE || bad_g;
+  p.gz = (d->act != LIN_NONE && (dx || dw)) || bad_g;
   p.w = pack && dx && !lin_dwords((const T*)w, d->k);
   p.x = pack && dw && !lin_dwords((const T*)x, d->ldx);
   p.ldg = p.gz ? pitch(d->n) : d->n;
