@@ -151,6 +151,25 @@ def test_bias_gradient_alone_needs_no_activation_gradient(dtype):
         assert 0 < need <= 1024 * 1024 * 4, need
 
 
+@pytest.mark.parametrize('rows,k,n,ldx,dx,dw,most', [
+    (10_000_000, 255, 1, 255, 0, 1, 160e6), (10_000_000, 255, 1, 255, 1, 1, 160e6),       # one output: 160 MB of g, 5 GB of x
+    (10_000_000, 1, 255, 1, 1, 1, 160e6), (50_000, 7, 9001, 7, 1, 1, 100e6),               # rows of x below a chunk: 5 GB, 0.9 GB of g
+    (9, 20_001, 20_001, 20_001, 0, 1, 3e5), (1_000_003, 333, 31, 333, 1, 0, 32e6),         # contractions inside their first tile
+    (100_003, 1001, 1003, (1 << 20) + 2, 0, 1, 100e6)])                                    # rows of x too far apart
+def test_no_copies_for_products_that_cannot_stream(rows, k, n, ldx, dx, dw, most):
+    """Odd bf16 rows are laid out anew only for a product that can then stream both operands."""
+    from vfdepth_amd import _lib
+    lib = _lib.load()
+    p = 1 << 40
+    got = lib.vfd_linear_bwd_workspace(ctypes.byref(_desc(rows=rows, k=k, n=n, ldx=ldx, dtype=1)), p, p, p, dx, dw)
+    assert got < most, got
+    even = 100_004, 1002, 1004, 1002                                             # and where it can: g, w and x
+    odd = 100_003, 1001, 1003, 1001
+    ws = [lib.vfd_linear_bwd_workspace(ctypes.byref(_desc(rows=r, k=k, n=n, ldx=l, dtype=1)), p, p, p, 1, 1)
+          for r, k, n, l in (even, odd)]
+    assert ws[1] >= 2 * (100_003 * 1008 + 1003 * 1008 + 100_003 * 1008) > ws[0]
+
+
 def test_descriptor_layout(tmp_path):
     import os
     import subprocess
@@ -308,6 +327,25 @@ def test_parts_of_the_gradient(act):
         y = KN.LinearAct.apply(*leaves, act)
         grads = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], g))
         _check([y] + [next(grads) if n else None for n in need], vals, tol)
+
+
+@gpu
+@pytest.mark.parametrize('act', ['none', 'silu'])
+@pytest.mark.parametrize('M,K,N', [(2_000_000, 255, 3), (2_000_000, 3, 255), (30_001, 7, 9001), (9, 13_001, 13_003), (200_003, 333, 31),
+                                   (40_001, 255, 257)])
+def test_odd_rows_of_short_products(M, K, N, act):
+    """Odd bf16 rows with one size below a chunk or a tile (no copies), and above (copies), enough terms for either: the last
+    rows and columns against the oracle, the weight's gradient of rows that are zero but for those."""
+    from vfdepth_amd import kernels as KN
+    x, w, b, _, g = _case(M, K, N, BF16, residual=False, seed=K)
+    g[:-300] = 0
+    y, dx, dw, db, _ = _run(x, w, b, None, g, act)
+    vals, tol = _oracle(x[-300:], w, b, None, g[-300:], act)
+    _check([y[-300:], dx[-300:], dw, db], vals, tol)
+    assert not dx[:-300].any()
+    dw2, = torch.autograd.grad(KN.LinearAct.apply(x.detach(), w, b.detach(), None, act), w, g)       # its copies alone
+    dx2, = torch.autograd.grad(KN.LinearAct.apply(x, w.detach(), b.detach(), None, act), x, g)
+    _check([None, dx2[-300:], dw2], vals, tol)
 
 
 @gpu

@@ -832,9 +832,10 @@ template <typename T>
 static bool lin_dwords(const T* p, long long ld) {
   return (((uintptr_t)p | (uintptr_t)ld * sizeof(T)) & 3) == 0;
 }
+constexpr long long LIN_LD = 1 << 20;
 template <typename T, bool MC>
 static bool lin_aligned(const LinOp<T>& op) {
-  return lin_dwords(op.p, op.ld) && (!MC || op.O >= LinT<T>::VE) && op.ld < (1 << 20);
+  return lin_dwords(op.p, op.ld) && (!MC || op.O >= LinT<T>::VE) && op.ld < LIN_LD;
 }
 
 // Which tiles a bf16 product takes.  Both measured with their contraction's length (one box, microseconds): a round of 256
@@ -945,16 +946,24 @@ static LinBwdPlan lin_bwd_plan(const vfd_linear_desc* d, const void* g, const vo
   auto pitch = [](long long n) { return (n + 63) / 64 * 64 * 16 <= n * 17 ? (n + 63) / 64 * 64 : (n + 7) / 8 * 8; };
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   LinBwdPlan p;
-  // a product of few terms is not worth copies of its operands (both gradients, with and without: 20 001 x 255 x 257 60 and
-  // 50 us, 2000 x 1001 x 1003 51 and 58)
-  const bool pack = (dx || dw) && (double)d->rows * d->k * d->n > 1.5e9;
-  const bool bad_g = pack && !lin_dwords((const T*)g, d->n);
-  p.gz = (d->act != LIN_NONE && (dx || dw)) || bad_g;
-  p.w = pack && dx && !lin_dwords((const T*)w, d->k);
-  p.x = pack && dw && !lin_dwords((const T*)x, d->ldx);
-  p.ldg = p.gz ? pitch(d->n) : d->n;
-  p.ldw = p.w ? pitch(d->k) : d->k;
-  p.ldx = p.x ? pitch(d->k) : d->ldx;
+  // A copy is made for a product whose operands can both be streamed with it (lin_aligned), for a whole tile of contraction at
+  // least: never for one of fewer than VE values a row, or of a contraction that ends inside its first tile (both gradients
+  // of 2 000 000 x 255 x 3 809 us and 1 MB of workspace, 2015 us and 1.06 GB with copies that nothing streamed).
+  // A product of few terms is not worth copies of its operands (both gradients, with and without: 20 001 x 255 x 257 60 and
+  // 50 us, 2000 x 1001 x 1003 51 and 58).
+  constexpr int VE = LinT<T>::VE, TILE = 64 / (int)sizeof(T);
+  const bool pack = (double)d->rows * d->k * d->n > 1.5e9;
+  const bool bad_g = !lin_dwords((const T*)g, d->n), bad_w = !lin_dwords((const T*)w, d->k), bad_x = !lin_dwords((const T*)x, d->ldx);
+  const long long ldg = d->act != LIN_NONE || bad_g ? pitch(d->n) : d->n, ldw = bad_w ? pitch(d->k) : d->k,
+                  ldx = bad_x ? pitch(d->k) : d->ldx;
+  const bool for_dx = pack && dx && d->n >= TILE && d->k >= VE && ldg < LIN_LD && ldw < LIN_LD;
+  const bool for_dw = pack && dw && d->rows >= TILE && d->n >= VE && d->k >= VE && ldg < LIN_LD && ldx < LIN_LD;
+  p.gz = (d->act != LIN_NONE && (dx || dw)) || (bad_g && (for_dx || for_dw));
+  p.w = bad_w && for_dx;
+  p.x = bad_x && for_dw;
+  p.ldg = p.gz ? ldg : d->n;
+  p.ldw = p.w ? ldw : d->k;
+  p.ldx = p.x ? ldx : d->ldx;
   p.at_gz = 0;
   p.at_w = p.at_gz + up(p.gz ? (size_t)d->rows * p.ldg * sizeof(T) : 0);
   p.at_x = p.at_w + up(p.w ? (size_t)d->n * p.ldw * sizeof(T) : 0);
