@@ -91,6 +91,19 @@ def _run(x, w, b, res, g, act):
     return [y] + [next(grads) if t is not None else None for t in (x, w, b, res)]
 
 
+def _near_product(got, a, b, what, extra=0.0):
+    """got against a @ b in 64 bits, for operands with random signs, tightly enough that a few missing terms show.  Of n
+    terms every partial sum is rounded, by at most u of itself: together at most u sum_k |S_k|.  The partial sums of terms
+    of random signs walk: |S_k| is some sqrt(sum of the terms' squares), 0.53 of it on average over k, over 3 of it on
+    average in no entry here; n + 8 counts the roundings of any order, splits and products among them."""
+    a, b = a.double(), b.double()
+    v = a @ b
+    e = 3 * (a.shape[1] + 8) * U * (a.square() @ b.square()).sqrt() + extra
+    err = (got.double() - v).abs()
+    lim = e + HALF[got.dtype] * (v.abs() + e) + TINY
+    assert got.shape == v.shape and bool((err <= lim).all()), (what, float((err / lim).max()))
+
+
 # ------------------------------------------------------------------------------------------------ CPU
 def _desc(rows=4, k=8, n=8, act=0, ldx=8, dtype=0):
     from vfdepth_amd import _lib
@@ -138,6 +151,23 @@ def test_c_refuses_null_tensors_and_small_workspaces():
     need = lib.vfd_linear_fwd_workspace(ctypes.byref(d))
     assert need > 0 and lib.vfd_linear_fwd(ctypes.byref(d), p, p, no, no, p, no, p, need - 1, no) == -1
     assert lib.vfd_linear_fwd(ctypes.byref(_desc(rows=0)), *[no] * 7, 0, no) == 0
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', [(18686, 584, 66), (16825, 143, 8), (17993, 8, 65), (9000, 72, 136), (300, 517, 771)])
+def test_product_bound_sees_missing_terms(M, K, N, dtype):
+    """The bound of the products' tests, on mistakes planted here: rows left out, added twice or taken from elsewhere, in one
+    32 x 32 block of the product alone."""
+    x, _, _, _, gz = _case(M, K, N, dtype, residual=False, seed=M, device='cpu')
+    good = gz.double().t() @ x.double()
+    _near_product(good.to(dtype), gz.t(), x, 'dw')
+    c = min(N, 32), min(K, 32)
+    a, b = gz[:, :c[0]].double(), x[:, :c[1]].double()
+    for wrong in (-a[-32:].t() @ b[-32:], a[:16].t() @ b[:16], a[64:96].t() @ (b[96:128] - b[64:96])):
+        bad = good.clone()
+        bad[:c[0], :c[1]] += wrong
+        with pytest.raises(AssertionError, match='dw'):
+            _near_product(bad.to(dtype), gz.t(), x, 'dw')
 
 
 @pytest.mark.parametrize('dtype', [0, 1])
@@ -270,6 +300,38 @@ FORMS = [(12687, 9, 193), (17993, 8, 65), (16825, 143, 8), (12431, 216, 528), (1
 def test_tile_forms(M, K, N, dtype):
     args = _case(M, K, N, dtype, seed=M)
     _check(_run(*args, 'elu'), *_oracle(*args, 'elu'))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('act', ['none', 'elu', 'gelu'])
+@pytest.mark.parametrize('M,K,N', SHAPES + FORMS + [(4200, 1160, 4104)])
+def test_products(M, K, N, act, dtype):
+    """Every product against 64 bits on the operands that it really took.  The pre-activation is what the layer without an
+    activation returns; its gradient is what a layer of unit weights gives back (times one and plus zeros: exact)."""
+    from vfdepth_amd import kernels as KN
+    x, w, b, _, g = _case(M, K, N, dtype, residual=False, seed=M + N)
+    y, dx, dw, db, _ = _run(x, w, b, None, g, act)
+    with torch.no_grad():
+        z = KN.LinearAct.infer(x, w, b, None, 'none')
+        zd, bd = x.double() @ w.double().t(), b.double()
+        _near_product(z, torch.cat([x, b.new_ones(M, 1)], 1), torch.cat([w, b[:, None]], 1).t(), 'z', U * (zd.abs() + bd.abs()))
+    gz = g
+    if act != 'none':
+        one = torch.eye(N, device='cuda', dtype=dtype)
+        gz, = torch.autograd.grad(KN.LinearAct.apply(z.requires_grad_(True), one, None, None, act), z, g)
+    with torch.no_grad():
+        gd = g.double()
+        _, slope, _ = _slope(z.double(), act)
+        exact = gd * slope
+        if act == 'none':
+            assert torch.equal(y, z)
+        else:
+            e = 8 * U * gd.abs() + U * exact.abs()
+            assert bool(((gz.double() - exact).abs() <= e + HALF[dtype] * (exact.abs() + e) + TINY).all())
+        _near_product(dx, gz, w, 'dx')
+        _near_product(dw, gz.t(), x, 'dw')
+        _near_product(db[None], torch.ones(1, M, device='cuda'), exact, 'db', 8 * U * gd.abs().sum(0) if act != 'none' else 0)
 
 
 @gpu
