@@ -73,6 +73,34 @@ def _ddp_worker(rank, world, port, q):
         raise
 
 
+def _clip_worker(rank, world, port, q):
+    sys.path.insert(0, ROOT)
+    try:
+        _init(rank, world, port)
+        from vfdepth_amd import config as C
+        from vfdepth_amd.layers import seeded_state_dict
+        from vfdepth_amd.vfdepth import VFDepthAlgo
+        cfg = C.mono_cfg(batch_size=1, height=64, width=96, max_grad_norm=1e-3)
+        cfg['ddp'].update({'ddp_enable': True, 'world_size': world, 'gpus': list(range(world))})
+        algo = VFDepthAlgo(cfg, 'cpu')
+        depth = algo.models['depth_net']
+        depth.module.load_state_dict(seeded_state_dict(depth.module, seed=3))
+        depth.eval()
+        x = torch.rand(1, 3, 64, 96, generator=torch.Generator().manual_seed(100 + rank))
+        sum(v.float().mean() for v in depth(x).values()).backward()
+        grads = [p.grad for p in depth.module.parameters() if p.grad is not None]
+        mean = torch.cat([g.flatten() for g in grads]).clone()       # averaged over the ranks by now
+        algo.clip_gradients()
+        after = torch.cat([g.flatten() for g in grads])
+        q.put((rank, float(algo.grad_norm), float(mean.double().norm()),
+               float((after.double() - mean.double() * (1e-3 / (mean.double().norm() + 1e-6))).abs().max() / mean.abs().max()),
+               float(after.double().sum())))
+        dist.destroy_process_group()
+    except Exception as e:                # surface the failure in the parent
+        q.put((rank, 'error', repr(e)))
+        raise
+
+
 def _bench_worker(rank, world, port, q):
     sys.path.insert(0, ROOT)
     _init(rank, world, port)
@@ -105,6 +133,13 @@ def test_ddp_gradient_allreduce_gloo_world2():
         assert all(sync_bn.values()), sync_bn          # CPU rehearsal: plain BatchNorm kept
         assert err <= 1e-6 * max(scale, 1e-12) + 1e-9, (rank, err, scale)   # DDP grad == mean of local grads
         assert peer == 0.0, (rank, peer)               # every rank holds the same averaged gradient
+
+
+def test_ddp_clipping_gloo_world2():
+    """training.max_grad_norm under DDP: every rank clips the averaged gradients, to one norm and one result."""
+    (_, n0, mean0, off0, sum0), (_, n1, mean1, off1, sum1) = _run(_clip_worker)
+    assert n0 == n1 and mean0 == mean1 > 1e-3 and sum0 == sum1, (n0, n1, mean0, mean1, sum0, sum1)
+    assert abs(n0 - mean0) <= 1e-5 * mean0 and max(off0, off1) <= 1e-5 * 1e-3 / mean0, (n0, mean0, off0, off1)
 
 
 def test_bench_job_time_is_max_over_ranks():

@@ -181,3 +181,21 @@ def test_ddp_graphed_step_world1_matches_eager(nccl_group):
         # the bitwise check is test_graph_replay_bit_identical[ddp_world1]
         assert rel <= max(1e-2, 4.0 * spread), \
             f'{net}: graph vs eager DDP gradient rel diff {rel:.3g} (eager vs eager {spread:.3g})'
+
+
+def test_ddp_step_clips_world1(nccl_group):
+    """training.max_grad_norm under DDP on the GPU: the reducer's gradients (views of its buckets or not) are clipped in
+    place between backward and the optimizer's step."""
+    from vfdepth_amd import kernels as KN
+    from vfdepth_amd import synth
+    from vfdepth_amd.vfdepth import VFDepthAlgo
+    cfg = G.step_cfg()
+    cfg['ddp'].update({'ddp_enable': True, 'world_size': 1, 'gpus': [0]})
+    cfg['training']['max_grad_norm'] = 1e-3
+    algo = VFDepthAlgo(cfg, 0)
+    algo.set_train()
+    for seed in (5, 6):
+        algo.train_step(dict(synth.make_batch(cfg, seed=seed, device=DEV)))
+        before = float(algo.grad_norm)
+        after = float(KN.grad_norm([p.grad for g in algo.optimizer.param_groups for p in g['params'] if p.grad is not None]))
+        assert before > 1e-3 and abs(after - 1e-3 * before / (before + 1e-6)) <= 1e-8

@@ -347,3 +347,61 @@ def test_training_step_clips():
     grads = [p.grad for g in algo.optimizer.param_groups for p in g['params'] if p.grad is not None]
     after = float(KN.grad_norm(grads))
     assert before > 1e-3 and abs(after - 1e-3 * before / (before + 1e-6)) <= 1e-3 * 1e-5
+
+
+@gpu
+@pytest.mark.parametrize('norm_type', [2.0, math.inf])
+@pytest.mark.parametrize('into', [False, True])
+def test_thousands_of_tensors(into, norm_type):
+    """More partial norms than every scaling block joins for itself (8192): they are joined first."""
+    from vfdepth_amd import kernels as KN
+    sizes = [i % 3 + 1 for i in range(8500)]
+    flat = torch.randn(sum(sizes), generator=torch.Generator().manual_seed(2)).cuda()
+    flat[-1] = 4.0                                           # the largest, in the last tensor
+    grads, before = list(flat.split(sizes)), flat.clone()
+    n = float(flat.double().norm(norm_type))
+    assert abs(float(KN.grad_norm(grads, norm_type)) - n) <= HALF[F32] * n * (1 + 1e-6)
+    outs = torch.full_like(flat, 7.0) if into else None
+    got = KN.clip_grads(grads, 0.25 * n, norm_type, out=None if outs is None else list(outs.split(sizes)))
+    assert abs(float(got) - n) <= HALF[F32] * n * (1 + 1e-6)
+    _near(flat if outs is None else outs, before.cpu().double() * (0.25 * n / (n + 1e-6)), 2 * HALF[F32] * (1 + 1e-6))
+    assert outs is None or torch.equal(flat, before)
+
+
+@gpu
+@pytest.mark.parametrize('over', [True, False])
+def test_captured_training_step_clips(over):
+    """A captured step with training.max_grad_norm: at every replay `step.grad_norm` is that batch's norm before clipping,
+    and the gradients that the optimizer takes have the limit's norm, or their own where it is under the limit."""
+    from vfdepth_amd import kernels as KN
+    from vfdepth_amd import synth
+    from vfdepth_amd.config import mono_cfg
+    from vfdepth_amd.vfdepth import VFDepthAlgo
+    limit = 1e-3 if over else 1e6
+    cfg = mono_cfg(max_grad_norm=limit, height=64, width=96)
+    algo = VFDepthAlgo(cfg, 0)
+    algo.set_train()
+    algo.set_optimizer(capturable=True)
+    batches = [synth.make_batch(cfg, seed=s, device='cuda') for s in (1, 2, 3)]
+    step = algo.graphed_train_step(batches[0], warmup=2)
+    params = [p for g in algo.optimizer.param_groups for p in g['params']]
+    norms = []
+    for k in (0, 1, 2, 0):
+        step(batches[k])
+        torch.cuda.synchronize()
+        before = float(step.grad_norm)
+        after = float(KN.grad_norm([p.grad for p in params if p.grad is not None]))       # eager work between replays
+        want = limit * before / (before + 1e-6) if over else before
+        assert before > 1e-3 and math.isfinite(before) and abs(after - want) <= want * (1e-5 if over else 2 * HALF[F32])
+        norms.append(before)
+    assert len(set(norms)) == len(norms)                     # other batches and weights: other norms
+
+
+def test_no_limit_leaves_no_norm():
+    from vfdepth_amd.config import mono_cfg
+    from vfdepth_amd.vfdepth import VFDepthAlgo
+    for cfg in (mono_cfg(height=32, width=64), mono_cfg(max_grad_norm=None, height=32, width=64)):
+        algo = VFDepthAlgo(cfg, 'cpu')
+        assert algo.max_grad_norm == 0.0
+        algo.clip_gradients()
+        assert algo.grad_norm is None
