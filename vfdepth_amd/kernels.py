@@ -2149,11 +2149,13 @@ def _once(fn):
     return staticmethod(backward)
 
 
+_is_tracing, _in_transform = torch._C._is_tracing, torch._C._are_functorch_transforms_active
+
+
 def seen_through():
     """Whether something has to see a call as torch's operators: a tracer that records it (it would keep only the output's
     allocation), a forward-mode level (the output would carry no tangent) or a functional transform."""
-    return (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
-            or torch._C._are_functorch_transforms_active())
+    return forward_ad._current_level >= 0 or _is_tracing() or _in_transform()
 
 
 def _param(t, x, dtype, shape, what):

@@ -147,16 +147,24 @@ def max_pool_stem(pool, x):
     return pool(x)
 
 
-_FORWARDS = {nn.LayerNorm.forward, nn.Linear.forward, nn.Conv2d.forward}
+_has_global_hook = torch.nn.modules.module._has_any_global_hook
+_FORWARDS = {t: t.forward for t in (nn.LayerNorm, nn.Linear, nn.Conv2d, ReflectConv2d)}
+
+
+def _inherits_forward(t):
+    return (t.forward in _FORWARDS.values()
+            and getattr(t, '_conv_forward', None) in (None, nn.Conv2d._conv_forward, ReflectConv2d._conv_forward))
 
 
 def _only_forward(m):
     """Whether calling module `m` is its class's forward and nothing else, so that a kernel may take its parameters
     instead: no hooks (weight normalisation computes the weight in one), no forward of a subclass or of the object."""
-    return (type(m).forward in _FORWARDS
-            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks
-                     or 'forward' in m.__dict__ or torch.nn.modules.module._has_any_global_hook())
-            and getattr(type(m), '_conv_forward', None) in (None, nn.Conv2d._conv_forward, ReflectConv2d._conv_forward))
+    t = type(m)
+    if _FORWARDS.get(t) is not t.forward and not _inherits_forward(t):
+        return False
+    d = m.__dict__
+    return not (d['_forward_pre_hooks'] or d['_forward_hooks'] or d['_backward_pre_hooks'] or d['_backward_hooks']
+                or 'forward' in d or _has_global_hook())
 
 
 def layer_norm(ln, x):
