@@ -260,3 +260,65 @@ def test_plain_modules_take_the_kernels():
         assert type(fn).__name__ == 'LinearActBackward'
     y = layers.layer_norm(torch.nn.LayerNorm(8).cuda(), torch.randn(3, 8, device='cuda'))
     assert type(y.grad_fn).__name__ == 'LayerNormBackward'
+
+
+def _relaid(t):
+    """The same values, stored the other way round: last dimension apart, rows beside each other."""
+    return t if t.dim() < 2 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('how', ['cpu', 'relaid', 'spread'])
+def test_saved_tensors_come_back_in_another_layout(how, dtype):
+    """Saved-tensor hooks (save_on_cpu packs densely) may change how far apart the saved rows lie: the gradients are those
+    of a backward without hooks, bit for bit."""
+    from vfdepth_amd import kernels as KN
+    graph = torch.autograd.graph
+    spread = lambda t: t if t.dim() < 2 else torch.nn.functional.pad(t, (3, 6))[..., 3:-6]  # noqa: E731
+    hooks = {'cpu': lambda: graph.save_on_cpu(), 'relaid': lambda: graph.saved_tensors_hooks(_relaid, lambda t: t),
+             'spread': lambda: graph.saved_tensors_hooks(spread, lambda t: t)}[how]
+    wide = torch.randn(150, 107, device='cuda').to(dtype)
+    w, b = torch.randn(40, 96, device='cuda').to(dtype), torch.randn(40, device='cuda').to(dtype)
+    ln_w = torch.randn(96, device='cuda')
+    for x in (wide[:, 5:101], wide[::3, 2:98], wide[:, :96].contiguous(), wide[:1, :96], wide[:96, :96].t()):
+        runs = []
+        for hooked in (False, True):
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, b, ln_w)]
+            xl, wl, bl, nl = leaves
+            with hooks() if hooked else torch.enable_grad():
+                y, z = KN.LinearAct.apply(xl, wl, bl, None, 'gelu'), KN.LayerNorm.apply(xl, nl, None, 1e-5)
+            gen = torch.Generator(device='cuda').manual_seed(7)
+            gy, gz = (torch.randn(t.shape, generator=gen, device='cuda').to(dtype) for t in (y, z))
+            runs.append(torch.autograd.grad(y, leaves[:3], gy) + torch.autograd.grad(z, (xl, nl), gz))
+        assert all(torch.equal(a, c) for a, c in zip(*runs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('change', [lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten()[:-1], lambda t: t.half()])
+def test_saved_tensors_that_come_back_as_others_are_refused(change):
+    from vfdepth_amd import kernels as KN
+    x, w = torch.randn(12, 8, device='cuda', requires_grad=True), torch.randn(6, 8, device='cuda', requires_grad=True)
+    lw = torch.randn(8, device='cuda', requires_grad=True)
+    for call, leaves in ((lambda: KN.LinearAct.apply(x, w, None, None, 'silu'), (x, w)), (lambda: KN.LayerNorm.apply(x, lw, None, 1e-5), (x, lw))):
+        with torch.autograd.graph.saved_tensors_hooks(change, lambda t: t):
+            y = call()
+        with pytest.raises(RuntimeError, match='saved-tensor hook'):
+            torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_checkpointed_block(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(4)
+    blk = Block(48, 100).cuda()
+    x = torch.randn(70, 48, device='cuda', requires_grad=True)
+    g = torch.randn(70, 48, device='cuda')
+    runs = []
+    for y in (lambda: blk(x), lambda: checkpoint(blk, x, use_reentrant=reentrant)):
+        for t in (x, *blk.parameters()):
+            t.grad = None
+        y().backward(g)
+        runs.append([t.grad for t in (x, *blk.parameters())])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -2167,9 +2167,31 @@ def _param(t, x, dtype, shape, what):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _as(t, like):
+_TYPES = (torch.float32, torch.bfloat16)          # of a descriptor's dtype
+
+
+def _as(t, dtype):
     """An incoming gradient, dense and of the forward's type."""
-    return t if t.dtype == like.dtype and t.is_contiguous() else t.to(like.dtype).contiguous()
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _saved(t, dtype, numel, g):
+    """A tensor that the forward saved, dense.  A saved-tensor hook may hand it back laid out anew; on another device, in
+    another type or size the kernels would read past its end."""
+    if t is None:
+        return None
+    if t.get_device() != g.get_device() or t.dtype != dtype or t.numel() != numel:
+        raise RuntimeError(f'saved: {numel} x {str(dtype)[6:]} on {g.device}, a saved-tensor hook returned {t.numel()} x '
+                           f'{str(t.dtype)[6:]} on {t.device}')
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _saved_rows(x, dtype, rows, cols, g, what):
+    """The saved input's rows, and how far apart they lie now."""
+    if x.get_device() != g.get_device() or x.dtype != dtype or x.numel() != rows * cols or x.shape[-1] != cols:
+        x = _saved(x, dtype, rows * cols, g).view(rows, cols)
+    x, _, ldx = _rows(x, what)
+    return x, ldx
 
 
 class LayerNorm(torch.autograd.Function):
@@ -2221,7 +2243,10 @@ class LayerNorm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         d = ctx.d
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        g = _as(g, x)
+        dtype = _TYPES[d.dtype]
+        g = _as(g, dtype)
+        x, d.ldx = _saved_rows(x, dtype, d.rows, d.cols, g, 'layer norm')
+        weight, stats = _saved(weight, torch.float32, d.cols, g), _saved(stats, torch.float32, 2 * d.rows, g)
         dx = torch.empty_like(g) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty(d.cols, dtype=torch.float32, device=g.device) if need_b else None
@@ -2304,7 +2329,10 @@ class LinearAct(torch.autograd.Function):
         dr = g if need_r else None
         if not (need_x or need_w or need_b):
             return None, None, None, dr, None
-        g = _as(g, x)
+        dtype = _TYPES[d.dtype]
+        g = _as(g, dtype)
+        x, d.ldx = _saved_rows(x, dtype, d.rows, d.k, g, 'linear')
+        weight, z = _saved(weight, dtype, d.n * d.k, g), _saved(z, dtype, d.rows * d.n, g)
         dx = torch.empty((*g.shape[:-1], d.k), dtype=g.dtype, device=g.device) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty(d.n, dtype=g.dtype, device=g.device) if need_b else None
