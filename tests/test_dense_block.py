@@ -136,6 +136,23 @@ def test_traced_block(grad):
 
 
 @pytest.mark.gpu
+def test_recorded_by_dispatch_modes():
+    """make_fx and torch.export record torch's operators; a mode that counts them counts the block's products."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    for m, shape in _recorded_cases():
+        x, z = torch.randn(shape, device='cuda'), torch.randn(shape, device='cuda')
+        with torch.no_grad():
+            want = _plain_block(m, z)
+            for fn in (make_fx(m)(x), torch.export.export(m, (x,)).module()):
+                assert torch.allclose(fn(z), want, rtol=1e-5, atol=1e-5)
+        with FlopCounterMode(display=False) as count:
+            m(x)
+        products = 2 * 2 * 5 * 24 * 40 if isinstance(m, Block) else 2 * 2 * 12 * 16 * 16
+        assert count.get_total_flops() == products
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('grad', [False, True])
 def test_forward_mode_and_functional_transforms(grad):
     """The tangent of a dual input is carried through, with a graph or without, and a transform sees the operators."""

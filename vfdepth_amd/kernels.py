@@ -2149,13 +2149,14 @@ def _once(fn):
     return staticmethod(backward)
 
 
-_is_tracing, _in_transform = torch._C._is_tracing, torch._C._are_functorch_transforms_active
+_is_tracing, _in_transform, _modes = (torch._C._is_tracing, torch._C._are_functorch_transforms_active,
+                                      torch._C._len_torch_dispatch_stack)
 
 
 def seen_through():
-    """Whether something has to see a call as torch's operators: a tracer that records it (it would keep only the output's
-    allocation), a forward-mode level (the output would carry no tangent) or a functional transform."""
-    return forward_ad._current_level >= 0 or _is_tracing() or _in_transform()
+    """Whether something has to see a call as torch's operators: a tracer or a dispatch mode that records it (it would keep
+    only the output's allocation), a forward-mode level (the output would carry no tangent) or a functional transform."""
+    return forward_ad._current_level >= 0 or _is_tracing() or _modes() > 0 or _in_transform()
 
 
 def _param(t, x, dtype, shape, what):

@@ -170,8 +170,8 @@ def _only_forward(m):
 def layer_norm(ln, x):
     """nn.LayerNorm `ln` over the last dimension of x [..., C]: the HIP kernel pair (layernorm.hip) for fp32 or bf16
     activations on the GPU (parameters and statistics fp32, the output in x's type), the module otherwise (CPU, other
-    types, several normalised dimensions; a module with hooks or a forward of its own; under torch.jit.trace, forward-mode
-    differentiation or a functional transform)."""
+    types, several normalised dimensions; a module with hooks or a forward of its own; under a tracer, a dispatch mode,
+    forward-mode differentiation or a functional transform)."""
     from . import kernels as KN
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not KN.seen_through() and _only_forward(ln)
             and len(ln.normalized_shape) == 1 and x.dim() >= 1 and x.shape[-1] == ln.normalized_shape[0]):
@@ -195,8 +195,8 @@ def linear_act(lin, x, act='none', residual=None):
     """act(lin(x)) + residual for `lin` an nn.Linear (x [..., K]) or a 1x1 nn.Conv2d (x a map [N, K, H, W]): the product
     with bias, activation and residual in its epilogue (linear.hip) for fp32 or bf16 on the GPU, under autocast in its
     type (a residual of another type is then added by torch, in the wider of the two); the module + torch ops otherwise
-    (CPU, other types; a module with hooks or a forward of its own; under torch.jit.trace, forward-mode differentiation
-    or a functional transform).  act: 'none', 'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The kernel's output for
+    (CPU, other types; a module with hooks or a forward of its own; under a tracer, a dispatch mode, forward-mode
+    differentiation or a functional transform).  act: 'none', 'relu', 'lrelu' (slope 0.1), 'elu', 'gelu', 'silu'.  The kernel's output for
     a convolution is channels-last; a channels-last map is read where it lies, another one is copied into that layout
     first."""
     if act not in _ACTS:
