@@ -917,8 +917,9 @@ static size_t lin_part_bytes(int M, int N, int K) {
   return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
 }
 
-// Row blocks of lin_act_bwd_k, 1024 blocks in all: with its column sums, 92 160 x 256 bf16 13.1 us, 15.9 with 2048 and 21.2 with
-// 4096; 16 384 x 8192 48.3, 51 and 55; 23 040 x 1024 fp32 18.4, 19.1 and 19.7.
+// Row blocks of lin_act_bwd_k, 1024 blocks in all.  Without an activation (g read, its blocks' sums written; the launch that
+// adds them, 4 to 5 us, is not counted): 92 160 x 256 bf16 13.1 us, 15.9 with 2048 and 21.2 with 4096; 16 384 x 8192 48.3, 51
+// and 55; 23 040 x 1024 fp32 18.4, 19.1 and 19.7.
 static int lin_strips(int M, int N, int V) {
   const int cb = (N + 64 * V - 1) / (64 * V), most = 1024 / cb > 0 ? 1024 / cb : 1, need = (M + 15) / 16;
   return need < most ? need : most;
