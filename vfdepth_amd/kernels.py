@@ -2176,22 +2176,29 @@ def _as(t, dtype):
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _saved(t, dtype, numel, g):
-    """A tensor that the forward saved, dense.  A saved-tensor hook may hand it back laid out anew; on another device, in
-    another type or size the kernels would read past its end."""
+def _saved(t, dtype, numel, device):
+    """A tensor that the forward saved, as it comes back: a saved-tensor hook may have laid it out anew.  On another device,
+    in another type or size the kernels would read past its end."""
+    if t.get_device() != device or t.dtype != dtype or t.numel() != numel:
+        raise RuntimeError(f'saved: {numel} x {str(dtype)[6:]} on cuda:{device}, a saved-tensor hook returned {t.numel()} x '
+                           f'{str(t.dtype)[6:]} on {t.device}')
+    return t
+
+
+def _saved_dense(t, dtype, numel, device):
     if t is None:
         return None
-    if t.get_device() != g.get_device() or t.dtype != dtype or t.numel() != numel:
-        raise RuntimeError(f'saved: {numel} x {str(dtype)[6:]} on {g.device}, a saved-tensor hook returned {t.numel()} x '
-                           f'{str(t.dtype)[6:]} on {t.device}')
-    return t if t.is_contiguous() else t.contiguous()
+    return _saved(t, dtype, numel, device) if t.is_contiguous() else _saved(t, dtype, numel, device).contiguous()
 
 
-def _saved_rows(x, dtype, rows, cols, g, what):
+def _saved_rows(x, dtype, rows, cols, device):
     """The saved input's rows, and how far apart they lie now."""
-    if x.get_device() != g.get_device() or x.dtype != dtype or x.numel() != rows * cols or x.shape[-1] != cols:
-        x = _saved(x, dtype, rows * cols, g).view(rows, cols)
-    x, _, ldx = _rows(x, what)
+    _saved(x, dtype, rows * cols, device)
+    if x.is_contiguous():
+        return x, cols
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+        return x, x.stride(0)
+    x, _, ldx = _rows(x, 'saved input')
     return x, ldx
 
 
@@ -2244,19 +2251,20 @@ class LayerNorm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         d = ctx.d
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dtype = _TYPES[d.dtype]
+        dtype, device, rows, cols = _TYPES[d.dtype], g.get_device(), d.rows, d.cols
         g = _as(g, dtype)
-        x, d.ldx = _saved_rows(x, dtype, d.rows, d.cols, g, 'layer norm')
-        weight, stats = _saved(weight, torch.float32, d.cols, g), _saved(stats, torch.float32, 2 * d.rows, g)
+        x, d.ldx = _saved_rows(x, dtype, rows, cols, device)
+        weight = _saved_dense(weight, torch.float32, cols, device)
+        stats = _saved_dense(stats, torch.float32, 2 * rows, device)
         dx = torch.empty_like(g) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty(d.cols, dtype=torch.float32, device=g.device) if need_b else None
+        db = torch.empty(cols, dtype=torch.float32, device=g.device) if need_b else None
         ws, nws = None, 0
         if need_w or need_b:
             nws = lib.vfd_layer_norm_bwd_workspace(d)
             ws = _ws(nws, g.device)
         m = stats.data_ptr()
-        L.check(lib.vfd_layer_norm_bwd(d, g.data_ptr(), x.data_ptr(), L.ptr(weight), m, m + 4 * d.rows, L.ptr(dx), L.ptr(dw),
+        L.check(lib.vfd_layer_norm_bwd(d, g.data_ptr(), x.data_ptr(), L.ptr(weight), m, m + 4 * rows, L.ptr(dx), L.ptr(dw),
                                        L.ptr(db), L.ptr(ws), nws, L.stream()), 'layer_norm_bwd')
         if L.PROF_ON:
             L.ALG_BYTES['layer_norm_bwd'] += (2 + need_x) * g.numel() * g.element_size()
@@ -2307,7 +2315,7 @@ class LinearAct(torch.autograd.Function):
             residual = _param(residual, x, dtype, shape, 'linear residual')
         x2, rows, ldx = _rows(x, 'linear')
         d = L.LinearDesc(rows, K, N, L.LINEAR_ACTS[act], ldx, code)
-        y = torch.empty(shape, dtype=dtype, device=x.device)
+        y = x.new_empty(shape)
         z = None
         if d.act and keep:
             z = torch.empty_like(y)
@@ -2330,13 +2338,14 @@ class LinearAct(torch.autograd.Function):
         dr = g if need_r else None
         if not (need_x or need_w or need_b):
             return None, None, None, dr, None
-        dtype = _TYPES[d.dtype]
+        dtype, device, rows, n, k = _TYPES[d.dtype], g.get_device(), d.rows, d.n, d.k
         g = _as(g, dtype)
-        x, d.ldx = _saved_rows(x, dtype, d.rows, d.k, g, 'linear')
-        weight, z = _saved(weight, dtype, d.n * d.k, g), _saved(z, dtype, d.rows * d.n, g)
-        dx = torch.empty((*g.shape[:-1], d.k), dtype=g.dtype, device=g.device) if need_x else None
+        x, d.ldx = _saved_rows(x, dtype, rows, k, device)
+        weight = _saved_dense(weight, dtype, n * k, device)
+        z = _saved_dense(z, dtype, rows * n, device)
+        dx = g.new_empty((*g.shape[:-1], k)) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty(d.n, dtype=g.dtype, device=g.device) if need_b else None
+        db = g.new_empty(n) if need_b else None
         pg, pw, px = g.data_ptr(), weight.data_ptr(), x.data_ptr()
         nws = lib.vfd_linear_bwd_workspace(d, pg, pw, px, need_x, need_w)
         ws = _ws(nws, g.device)

@@ -175,7 +175,11 @@ def layer_norm(ln, x):
     from . import kernels as KN
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and not KN.seen_through() and _only_forward(ln)
             and len(ln.normalized_shape) == 1 and x.dim() >= 1 and x.shape[-1] == ln.normalized_shape[0]):
-        w, b = (p if p is None or p.dtype == torch.float32 else p.float() for p in (ln.weight, ln.bias))
+        w, b = ln.weight, ln.bias
+        if w is not None and w.dtype != torch.float32:
+            w = w.float()
+        if b is not None and b.dtype != torch.float32:
+            b = b.float()
         return (KN.LayerNorm.apply if torch.is_grad_enabled() else KN.LayerNorm.infer)(x, w, b, ln.eps)
     return ln(x)
 
