@@ -260,6 +260,21 @@ def test_global_hooks_see_the_modules(device):
     assert seen == [ln, lin]
 
 
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_scripted_modules_and_other_callables(device):
+    """What is no ordinary module is called, on either device."""
+    import warnings
+    from vfdepth_amd import layers
+    lin, ln = torch.nn.Linear(6, 4).to(device), torch.nn.LayerNorm(6).to(device)
+    x = torch.randn(3, 6, device=device)
+    with warnings.catch_warnings():
+        warnings.simplefilter('ignore')
+        scripted = torch.jit.script(lin), torch.jit.script(ln)
+    for a, b in (scripted, (lambda t: lin(t), lambda t: ln(t))):
+        assert torch.allclose(layers.linear_act(a, x, 'relu'), torch.relu(lin(x)), rtol=1e-5, atol=1e-5)
+        assert torch.allclose(layers.layer_norm(b, x), ln(x), rtol=1e-5, atol=1e-5)
+
+
 @pytest.mark.gpu
 def test_plain_modules_take_the_kernels():
     """Ordinary modules, a subclass without a forward and a parametrized weight are not sent to the module."""

@@ -152,7 +152,7 @@ _FORWARDS = {t: t.forward for t in (nn.LayerNorm, nn.Linear, nn.Conv2d, ReflectC
 
 
 def _inherits_forward(t):
-    return (t.forward in _FORWARDS.values()
+    return (getattr(t, 'forward', None) in _FORWARDS.values()
             and getattr(t, '_conv_forward', None) in (None, nn.Conv2d._conv_forward, ReflectConv2d._conv_forward))
 
 
@@ -160,7 +160,8 @@ def _only_forward(m):
     """Whether calling module `m` is its class's forward and nothing else, so that a kernel may take its parameters
     instead: no hooks (weight normalisation computes the weight in one), no forward of a subclass or of the object."""
     t = type(m)
-    if _FORWARDS.get(t) is not t.forward and not _inherits_forward(t):
+    known = _FORWARDS.get(t)
+    if (known is None or known is not t.forward) and not _inherits_forward(t):
         return False
     d = m.__dict__
     return not (d['_forward_pre_hooks'] or d['_forward_hooks'] or d['_backward_pre_hooks'] or d['_backward_hooks']
